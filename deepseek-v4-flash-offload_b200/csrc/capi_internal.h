@@ -19,6 +19,22 @@ int fail(int code, const std::string& msg);
 // (the library links its own runtime, so it does not see the caller's
 // cudaSetDevice).  Optionally returns the device ordinal.
 int bind_device_of(const void* ptr, int* device);
+// The device of `ptr` made current until the end of the scope, then the
+// caller's device again (for entry points called from code that keeps its own
+// current device).
+struct DeviceScope {
+  int prev = -1;
+  int enter(const void* ptr) {
+    int cur = -1, dev = -1;
+    if (cudaGetDevice(&cur) != cudaSuccess) cur = -1;
+    if (int rc = bind_device_of(ptr, &dev)) return rc;
+    if (cur >= 0 && cur != dev) prev = cur;
+    return DSV4_OK;
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no
 // libcuda link): rank-D map over `base` with element strides of 1.
 int make_map(CUtensorMap* m, CUtensorMapDataType dt, int rank, void* base, const uint64_t* dims,
@@ -59,6 +75,11 @@ int route_fused_launch(const void* x_bf16, const float* gate_w, const float* bia
 inline int64_t route_fused_part_bytes(int64_t n_tokens, int hidden, int n_experts) {
   return (int64_t)(hidden / 128) * n_tokens * n_experts * 4;
 }
+
+// act_quant with separate outputs (fp8_quant.cu): codes [rows, ldq], scales
+// [rows, ceil(cols / 128)].
+int act_quant_fp8_launch(const void* x, int x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q, int64_t ldq,
+                         void* scale, int scale_type, cudaStream_t st);
 
 // Byte layout of one packed expert slot (see include/dsv4moe.h).
 struct SlotLayout {

@@ -24,6 +24,9 @@ DSV4_EUNSUPPORTED = -7
 
 SCORE_FUNCS = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 PROFILES = {"bf16": 0, "a4w4": 1}
+# element types and FP8 scale types (DSV4_DT_*, DSV4_SCALE_*)
+DT_BF16, DT_FP16, DT_FP32 = 0, 1, 2
+SCALE_E8M0, SCALE_FP32, SCALE_FP32_POW2 = 0, 1, 2
 # token row formats of the expert-parallel dispatch (DSV4_ROWS_*)
 ROWS_BF16, ROWS_FP8, ROWS_MXFP4 = 0, 1, 2
 
@@ -40,6 +43,13 @@ SIGNATURES = {
     "dsv4_slot_dequant": (C.c_int, [_p, _i32, _i32, _p, _p, _p, _p]),
     "dsv4_act_quant_fp8_rt": (C.c_int, [_p, _i64, _i64, _p]),
     "dsv4_act_quant_mxfp4": (C.c_int, [_p, _i64, _i64, _p, _p, _p]),
+    "dsv4_act_quant_fp8": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i32, _p]),
+    "dsv4_fp8_matmul": (C.c_int, [_p, _i64, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _i64, _p, _i64, _i32, _p]),
+    "dsv4_fp8_status": (C.c_int, [_i32, _p]),
+    "dsv4_balance_workspace_bytes": (_i64, [_i64, _i32, _i32]),
+    "dsv4_balance_forward": (C.c_int, [_p, _i32, _i64, _i32, _p, _i32, _p, _i32, _i32, _f32, _p, _p, _p, _i64, _p,
+                                       _p]),
+    "dsv4_balance_backward": (C.c_int, [_p, _i32, _i64, _i32, _i32, _i32, _f32, _p, _p, _p, _i64, _p]),
     "dsv4_route_workspace_bytes": (_i64, [_i64, _i32, _i32]),
     "dsv4_route_topk": (C.c_int, [_p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _f32, _p, _p, _p,
                                   _i64, _p]),

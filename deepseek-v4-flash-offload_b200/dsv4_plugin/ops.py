@@ -3,11 +3,14 @@
 | here                    | reference                                           |
 |-------------------------|-----------------------------------------------------|
 | ``dequant_fp4_weight``  | npu_ops.dequant_fp4_weight (npu_ops.py:142-158)     |
-| ``act_quant``           | npu_ops.act_quant, inplace form (npu_ops.py:73-98)  |
+| ``act_quant``           | npu_ops.act_quant (npu_ops.py:73-104)               |
+| ``fp8_matmul``,         | a dense layer on a checkpoint's FP8 weight          |
+| ``fp8_linear``          | (npu_ops.dequant_fp8_weight, npu_ops.py:161-167)    |
 | ``dynamic_mx_quant``    | torch_npu.npu_dynamic_mx_quant (deepseek_v4.py:212) |
 | ``route_topk``          | OffloadDeepseekV4MoE._route (deepseek_v4.py:118-148)|
 | ``moe_align``           | the align block of _routed (deepseek_v4.py:154-164) |
 | ``MoEPlan.forward``     | _routed / _routed_mxfp4 (deepseek_v4.py:150-245)    |
+| ``balance_loss``        | none (the reference's router only serves)           |
 
 All tensors must live on a CUDA device; work runs on the current torch
 stream.  There is no CPU path.
@@ -19,9 +22,12 @@ import ctypes as C
 
 import torch
 
-from ._lib import PROFILES, ROWS_BF16, ROWS_FP8, ROWS_MXFP4, SCORE_FUNCS, check, lib  # noqa: F401
+from ._lib import (DT_BF16, DT_FP16, DT_FP32, PROFILES, ROWS_BF16, ROWS_FP8, ROWS_MXFP4,  # noqa: F401
+                   SCALE_E8M0, SCALE_FP32, SCALE_FP32_POW2, SCORE_FUNCS, check, lib)
 
 _E8M0 = getattr(torch, "float8_e8m0fnu", None)
+_E4M3 = torch.float8_e4m3fn
+_DT = {torch.bfloat16: DT_BF16, torch.float16: DT_FP16, torch.float32: DT_FP32}
 
 
 def _stream(dev: torch.device) -> int:
@@ -52,18 +58,206 @@ def dequant_fp4_weight(w_packed: torch.Tensor, scale: torch.Tensor, out_dtype=to
     return out
 
 
-def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt: str = "ue8m0", scale_dtype=None,
+def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt: str | None = "ue8m0", scale_dtype=None,
               inplace: bool = False):
-    """FP8-E4M3 round trip per 128 with a power-of-two scale, in place.
+    """FP8-E4M3 quantisation per row and 128 columns.
 
-    Only the in-place form used by the routed-expert path is provided."""
-    if not inplace or block_size != 128 or scale_fmt != "ue8m0":
-        raise NotImplementedError("only act_quant(x, 128, 'ue8m0', _, inplace=True) is provided")
+    ``inplace=True``: the round trip of a contiguous bf16 ``x`` with
+    power-of-two scales, in place; returns ``x``.
+
+    ``inplace=False``: (q, s) with q E4M3 of ``x``'s shape and s [..,
+    ceil(C / 128)].  ``x`` is bf16, fp16 or fp32, with any number of columns.
+    ``scale_fmt="ue8m0"``: the smallest power of two that brings the block
+    within 448, as ``scale_dtype`` float32 (also None) or float8_e8m0fnu;
+    ``scale_fmt=None``: amax / 448 in float32.  amax is at least 1e-4.  A NaN
+    stays NaN and leaves its block's scale alone; an infinity saturates."""
+    if block_size != 128 or scale_fmt not in ("ue8m0", None):
+        raise NotImplementedError("act_quant provides block_size 128 and scale_fmt 'ue8m0' or None")
+    if inplace:
+        if scale_fmt != "ue8m0":
+            raise NotImplementedError("only act_quant(x, 128, 'ue8m0', _, inplace=True) is provided in place")
+        _need_cuda(x)
+        if x.dtype != torch.bfloat16 or not x.is_contiguous():
+            raise TypeError("act_quant expects a contiguous bf16 tensor")
+        check(lib().dsv4_act_quant_fp8_rt(x.data_ptr(), x.numel() // x.shape[-1], x.shape[-1], _stream(x.device)))
+        return x
+    if x.dtype not in _DT:
+        raise TypeError(f"act_quant expects bf16, fp16 or fp32, got {x.dtype}")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("act_quant needs at least one column")
+    if scale_dtype not in (None, torch.float32) and (_E8M0 is None or scale_dtype != _E8M0 or scale_fmt is None):
+        raise TypeError("scale_dtype must be float32, or float8_e8m0fnu with scale_fmt 'ue8m0'")
     _need_cuda(x)
-    if x.dtype != torch.bfloat16 or not x.is_contiguous():
-        raise TypeError("act_quant expects a contiguous bf16 tensor")
-    check(lib().dsv4_act_quant_fp8_rt(x.data_ptr(), x.numel() // x.shape[-1], x.shape[-1], _stream(x.device)))
-    return x
+    x = x.detach().contiguous()
+    cols = x.shape[-1]
+    rows = x.numel() // cols
+    kind = SCALE_FP32 if scale_fmt is None else (SCALE_E8M0 if scale_dtype == _E8M0 else SCALE_FP32_POW2)
+    q = torch.empty(x.shape, dtype=_E4M3, device=x.device)
+    s = torch.empty((*x.shape[:-1], (cols + 127) // 128), dtype=_E8M0 if kind == SCALE_E8M0 else torch.float32,
+                    device=x.device)
+    check(lib().dsv4_act_quant_fp8(x.data_ptr(), _DT[x.dtype], rows, cols, cols, q.data_ptr(), cols, s.data_ptr(), kind,
+                                   _stream(x.device)))
+    return q, s
+
+
+def _fp8_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """(FP8 matrix the kernels can read, its row stride in bytes): rows that
+    start on 16 bytes, columns next to each other; copied when it is not."""
+    r, c = t.shape
+    ld = t.stride(0) if r > 1 else (c + 15) // 16 * 16
+    if (t.stride(1) == 1 or c == 1) and ld % 16 == 0 and ld >= c and t.data_ptr() % 16 == 0:
+        return t, ld
+    ld = (c + 15) // 16 * 16
+    p = torch.empty((r, ld), dtype=torch.uint8, device=t.device)
+    p[:, :c].copy_(t.contiguous().view(torch.uint8))
+    return p, ld
+
+
+def _fp8_scale(s: torch.Tensor) -> torch.Tensor:
+    """Scales as the kernels read them: contiguous E8M0 bytes or float32."""
+    return s.contiguous() if s.dtype == torch.float32 else _u8(s)
+
+
+def _is_e8m0(s: torch.Tensor) -> bool:
+    if s.dtype == torch.float32:
+        return False
+    if s.dtype == torch.uint8 or (_E8M0 is not None and s.dtype == _E8M0):
+        return True
+    raise TypeError(f"FP8 scales are float32 or E8M0 (float8_e8m0fnu or uint8), got {s.dtype}")
+
+
+def _e8m0_float(s: torch.Tensor) -> torch.Tensor:
+    return (s.view(_E8M0) if s.dtype == torch.uint8 else s).float()
+
+
+def _same_device(*ts):
+    _need_cuda(*ts)
+    if len({t.device for t in ts if t is not None}) > 1:
+        raise ValueError("the tensors live on different devices")
+
+
+def _check_fp8_weight(b: torch.Tensor, b_scale: torch.Tensor):
+    if b.dtype != _E4M3:
+        raise TypeError(f"expected a float8_e4m3fn matrix, got {b.dtype}")
+    if b.dim() != 2 or tuple(b_scale.shape) != ((b.shape[0] + 127) // 128, (b.shape[1] + 127) // 128):
+        raise ValueError(f"a matrix of shape {tuple(b.shape)} needs one scale per 128 x 128 block, "
+                         f"got {tuple(b_scale.shape)}")
+
+
+def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, trans_b: bool = True,
+               out_dtype=torch.bfloat16) -> torch.Tensor:
+    """Product of E4M3 matrices with a scale for each row and 128 of K of ``a``
+    ([.., K], a_scale [.., ceil(K / 128)]) and each 128 x 128 block of ``b``
+    ([N, K]; with ``trans_b=False`` [K, N]; b_scale one per block):
+    dequant(a) @ dequant(b).T (or @ dequant(b)) with fp32 sums, in bf16 or
+    fp32.  Scales: float32 or E8M0 (float8_e8m0fnu or uint8); where the two
+    differ, both are taken as float32.  No gradient: see ``fp8_linear``.
+
+    Rows of ``a`` and ``b`` may be strided.  Where they do not start on 16
+    bytes the matrix is copied first."""
+    if a.dtype != _E4M3:
+        raise TypeError(f"expected a float8_e4m3fn matrix, got {a.dtype}")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("out_dtype must be bfloat16 or float32")
+    _check_fp8_weight(b, b_scale)
+    if a.dim() < 1 or a.shape[-1] == 0:
+        raise ValueError("fp8_matmul needs K > 0")
+    k = a.shape[-1]
+    n, kb = (b.shape[0], b.shape[1]) if trans_b else (b.shape[1], b.shape[0])
+    if kb != k:
+        raise ValueError(f"a has K = {k}, b has K = {kb}")
+    if tuple(a_scale.shape) != (*a.shape[:-1], (k + 127) // 128):
+        raise ValueError(f"a_scale must be {(*a.shape[:-1], (k + 127) // 128)}, got {tuple(a_scale.shape)}")
+    e8 = _is_e8m0(a_scale)
+    if e8 != _is_e8m0(b_scale):
+        a_scale, b_scale = (_e8m0_float(a_scale), b_scale) if e8 else (a_scale, _e8m0_float(b_scale))
+        e8 = False
+    _same_device(a, a_scale, b, b_scale)
+    dev = a.device
+    y = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=dev)
+    m = y.numel() // n if n else 0
+    if m == 0:
+        return y
+    a2, lda = _fp8_rows(a if a.dim() == 2 else a.reshape(m, k))
+    b2, ldb = _fp8_rows(b)
+    sa, sb = _fp8_scale(a_scale), _fp8_scale(b_scale)
+    check(lib().dsv4_fp8_matmul(a2.data_ptr(), lda, sa.data_ptr(), b2.data_ptr(), ldb, sb.data_ptr(),
+                                SCALE_E8M0 if e8 else SCALE_FP32, int(bool(trans_b)), m, n, k, y.data_ptr(), n,
+                                _DT[out_dtype], _stream(dev)))
+    return y
+
+
+def fp8_status(device=None) -> None:
+    """Synchronise the current stream of ``device`` and raise if a wait of an
+    ``fp8_matmul`` / ``fp8_linear`` kernel ran out since the last call (its
+    outputs are then undefined)."""
+    dev = torch.device("cuda" if device is None else device)
+    if dev.type != "cuda":
+        raise ValueError("fp8_status needs a CUDA device")
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    check(lib().dsv4_fp8_status(index, _stream(dev)))
+
+
+def _fp8_linear_call(x: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, trans: bool) -> torch.Tensor:
+    """act_quant(x) times w (trans: w.T) -> x's type; scales of w's type."""
+    k = x.shape[-1]
+    n = w.shape[0] if trans else w.shape[1]
+    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    m = y.numel() // n if n else 0
+    if m == 0:
+        return y
+    x = x.detach().contiguous()
+    e8 = _is_e8m0(ws)
+    w2, ldw = _fp8_rows(w)
+    sw = _fp8_scale(ws)
+    st = _stream(x.device)
+    # codes (rows padded to 16 bytes), then the scales
+    ld = (k + 15) // 16 * 16
+    nb = (k + 127) // 128
+    buf = torch.empty(m * ld + m * nb * (1 if e8 else 4), dtype=torch.uint8, device=x.device)
+    q, s = buf.data_ptr(), buf.data_ptr() + m * ld
+    kind = SCALE_E8M0 if e8 else SCALE_FP32
+    dt = _DT[x.dtype]
+    check(lib().dsv4_act_quant_fp8(x.data_ptr(), dt, m, k, k, q, ld, s, kind, st))
+    check(lib().dsv4_fp8_matmul(q, ld, s, w2.data_ptr(), ldw, sw.data_ptr(), kind, int(trans), m, n, k, y.data_ptr(), n,
+                                dt, st))
+    return y
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, ws):
+        ctx.save_for_backward(w, ws)
+        return _fp8_linear_call(x, w, ws, True)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        w, ws = ctx.saved_tensors
+        return _fp8_linear_call(dy, w, ws, False), None, None
+
+
+def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
+    """Linear layer on a frozen FP8 weight [N, K] with one scale per 128 x 128
+    block: ``act_quant(x)`` (power-of-two scales for an E8M0 ``weight_scale``,
+    amax / 448 for a float32 one), then ``fp8_matmul``.  ``x`` [.., K] is bf16
+    or fp32, and so is the result [.., N].
+
+    Differentiable in ``x``: the gradient dy is quantised the same way, along
+    N, and multiplied with the same stored weight (the rounding of x is passed
+    through).  The weight is a checkpoint's and gets no gradient."""
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"fp8_linear expects bf16 or fp32, got {x.dtype}")
+    _check_fp8_weight(weight, weight_scale)
+    if weight.requires_grad or weight_scale.requires_grad:
+        raise ValueError("fp8_linear has no gradient for the weight or its scales")
+    if x.dim() == 0 or x.shape[-1] != weight.shape[1] or x.shape[-1] == 0:
+        raise ValueError(f"x {tuple(x.shape)} does not match the weight {tuple(weight.shape)}")
+    _is_e8m0(weight_scale)
+    _same_device(x, weight, weight_scale)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Fp8Linear.apply(x, weight, weight_scale)
+    return _fp8_linear_call(x, weight, weight_scale, True)
 
 
 def dynamic_mx_quant(x: torch.Tensor):
@@ -151,6 +345,85 @@ def moe_align(indices: torch.Tensor, n_experts: int) -> dict:
     out["sorted_flat"] = out["sorted_flat"][:p]
     out["inv"] = out["inv"][:p]
     return out
+
+
+class _BalanceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, indices, offsets, n_seqs, score, alpha, status):
+        t, e = logits.shape
+        dev = logits.device
+        logits = logits.detach().contiguous()
+        ws = torch.empty(int(lib().dsv4_balance_workspace_bytes(t, e, n_seqs)), dtype=torch.uint8, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        counts = torch.empty((n_seqs, e), dtype=torch.int32, device=dev)
+        check(lib().dsv4_balance_forward(logits.data_ptr(), _DT[logits.dtype], t, e, indices.data_ptr(),
+                                         indices.shape[1], None if offsets is None else offsets.data_ptr(), n_seqs,
+                                         score, alpha, loss.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(),
+                                         None if status is None else status.data_ptr(), _stream(dev)))
+        ctx.save_for_backward(logits, ws)
+        ctx.args = (n_seqs, score, alpha)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, _):
+        logits, ws = ctx.saved_tensors
+        n_seqs, score, alpha = ctx.args
+        t, e = logits.shape
+        up = grad_loss.float().contiguous()
+        out = torch.empty_like(logits)
+        check(lib().dsv4_balance_backward(logits.data_ptr(), _DT[logits.dtype], t, e, n_seqs, score, alpha,
+                                          up.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                          _stream(logits.device)))
+        return out, None, None, None, None, None, None
+
+
+def balance_loss(logits: torch.Tensor, indices: torch.Tensor, score_func: str = "sqrtsoftplus", alpha: float = 1.0,
+                 seq_offsets: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Load balance loss of a router (float32 scalar, differentiable in
+    ``logits``) and the picks per expert (int32 [E], or [S, E] with
+    ``seq_offsets``, which ``parallel_ep.balanced_placement`` takes as loads).
+
+    ``logits`` [T, E] fp32 or bf16 (E <= 1024), ``indices`` [T, k] the
+    router's picks (``route_topk``; -1 = empty).  ``seq_offsets`` [S + 1]
+    (integer, ascending, on the device) packs S sequences: rows o[s] ..
+    o[s+1]-1 are sequence s.  A row without a pick and a row outside the
+    sequences are padding: they do not count and their gradient is 0.  With p
+    = score / sum score, the picks c and the tokens n of a sequence:
+        alpha * mean_s sum_e (c[e] E / sum c) * (sum_t p[t, e] / n)
+    over the sequences that have tokens; the counts are constants of the
+    gradient.  A pick outside [-1, E) is skipped; it and offsets that descend
+    or leave [0, T] set DSV4_EINVAL (-1) in ``status`` (int32 [1], zeroed by
+    the caller) when it is given."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError("logits must be fp32 or bf16 [T, E]")
+    t, e = logits.shape
+    if not 1 <= e <= 1024:
+        raise ValueError("balance_loss handles 1 to 1024 experts")
+    if indices.dim() != 2 or indices.shape[0] != t or indices.shape[1] < 1:
+        raise ValueError("indices must be [T, k], one row per row of logits")
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError("indices must be int32 or int64")
+    if score_func not in SCORE_FUNCS:
+        raise ValueError(f"score_func must be one of {sorted(SCORE_FUNCS)}")
+    n_seqs = 1
+    if seq_offsets is not None:
+        if seq_offsets.dim() != 1 or seq_offsets.numel() < 2 or seq_offsets.dtype not in (torch.int32, torch.int64):
+            raise ValueError("seq_offsets must be int32 or int64 [S + 1] with S >= 1")
+        n_seqs = seq_offsets.numel() - 1
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+        raise TypeError("status must be an int32 tensor")
+    _same_device(logits, indices, seq_offsets, status)
+    if indices.dtype == torch.int64:
+        indices = indices.clamp(-2, e).to(torch.int32)     # what is out of range stays out of range
+    if seq_offsets is not None:
+        if seq_offsets.dtype == torch.int64:
+            seq_offsets = seq_offsets.clamp(-1, 0x7fffffff).to(torch.int32)
+        seq_offsets = seq_offsets.contiguous()
+    loss, counts = _BalanceLoss.apply(logits, indices.contiguous(), seq_offsets, n_seqs, SCORE_FUNCS[score_func],
+                                      float(alpha), status)
+    return loss, counts if seq_offsets is not None else counts[0]
 
 
 def combine_ordered(rows: torch.Tensor, order: torch.Tensor) -> torch.Tensor:

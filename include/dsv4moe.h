@@ -100,6 +100,77 @@ int dsv4_act_quant_mxfp4(const void* x_bf16, int64_t rows, int64_t cols, uint8_t
                          void* stream);
 
 /* ------------------------------------------------------------------------ *
+ * FP8 with a scale per block of 128: the checkpoint form of the dense
+ * weights (E4M3, one scale per 128 x 128 block; dequant_fp8_weight,
+ * npu_ops.py:161-167) and of the activations that meet them (act_quant,
+ * inplace=False; npu_ops.py:73-104).
+ *
+ * dsv4_act_quant_fp8: x [rows, cols] with row stride ldx (elements) -> E4M3
+ * q, row stride ldq bytes, and scale [rows, ceil(cols / 128)].  Per row and
+ * 128 columns a = max(1e-4, max |x|):
+ *   DSV4_SCALE_E8M0 / DSV4_SCALE_FP32_POW2: 2^e, the smallest e with
+ *     a <= 448 * 2^e, as the byte e + 127 or as fp32;
+ *   DSV4_SCALE_FP32: a / 448.
+ * q is the E4M3 value nearest to x / scale (for DSV4_SCALE_FP32: to
+ * 448 x / a).  NaN stays NaN and is left out of a; an infinity counts as the
+ * largest finite value and saturates.
+ *
+ * dsv4_fp8_matmul: y [m, n] (row stride ldy elements, bf16 or fp32) of a
+ * [m, k] (row stride lda bytes) with a_scale [m, ceil(k / 128)] and
+ *   trans_b != 0: b [n, k], b_scale [ceil(n / 128), ceil(k / 128)];
+ *   trans_b == 0: b [k, n], b_scale [ceil(k / 128), ceil(n / 128)],
+ * row stride ldb bytes; both scales E8M0 bytes or both fp32.  fp32 sums.  a
+ * and b start on 16 bytes with row strides that are multiples of 16; k, m
+ * and n are any size.
+ * A device-side wait that runs out is reported by dsv4_fp8_status.
+ * ------------------------------------------------------------------------ */
+#define DSV4_DT_BF16 0
+#define DSV4_DT_FP16 1
+#define DSV4_DT_FP32 2
+#define DSV4_SCALE_E8M0 0
+#define DSV4_SCALE_FP32 1
+#define DSV4_SCALE_FP32_POW2 2
+int dsv4_act_quant_fp8(const void* x, int32_t x_dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q,
+                       int64_t ldq, void* scale, int32_t scale_type, void* stream);
+int dsv4_fp8_matmul(const uint8_t* a, int64_t lda, const void* a_scale, const uint8_t* b, int64_t ldb,
+                    const void* b_scale, int32_t scale_type, int32_t trans_b, int64_t m, int64_t n, int64_t k, void* y,
+                    int64_t ldy, int32_t out_dtype, void* stream);
+/* Synchronises `stream`; returns and clears the device's FP8 status word (0,
+ * or DSV4_ETIMEOUT: the outputs since the last call are undefined). */
+int dsv4_fp8_status(int32_t device, void* stream);
+
+/* ------------------------------------------------------------------------ *
+ * Load balance loss of a router and its per-expert counts (no counterpart in
+ * the reference, which only serves; score functions as in
+ * OffloadDeepseekV4MoE._route, deepseek_v4.py:126-131).
+ * Rows seq_offsets[s] .. seq_offsets[s+1]-1 are sequence s (int32 [n_seqs +
+ * 1], ascending; NULL: one sequence of all rows); other rows belong to none.
+ * indices [n_tokens, topk] are the router's picks, -1 = empty; a row without
+ * a pick is padding.  Neither padding nor rows outside the sequences count.
+ * With p = score / sum_e score, c[s, e] the picks of expert e and n[s] the
+ * tokens of sequence s, f[s, e] = c[s, e] * n_experts / sum_e c[s, e]:
+ *   loss = alpha * mean over sequences with tokens of
+ *          sum_e f[s, e] * (1 / n[s]) * sum_t p[t, e];
+ * counts [n_seqs, n_experts] = c.  A row whose scores are all 0 has p = 0; a
+ * NaN or an infinite score makes the loss and its row's gradient NaN.  Picks
+ * outside [-1, n_experts) are skipped, and like offsets that descend or
+ * leave [0, n_tokens] they set DSV4_EINVAL in *status (device word, may be
+ * NULL).  logits are fp32 or bf16 [n_tokens, n_experts], n_experts <= 1024.
+ * The forward leaves in the workspace what the backward reads: dlogits (type
+ * of the logits, every row written, rows that do not count as zeros) =
+ * *grad_loss (device) times the gradient with the counts held constant.
+ * Results do not depend on scheduling.
+ * ------------------------------------------------------------------------ */
+int64_t dsv4_balance_workspace_bytes(int64_t n_tokens, int32_t n_experts, int32_t n_seqs);
+int dsv4_balance_forward(const void* logits, int32_t dtype, int64_t n_tokens, int32_t n_experts,
+                         const int32_t* indices, int32_t topk, const int32_t* seq_offsets, int32_t n_seqs,
+                         int32_t score_func, float alpha, float* loss, int32_t* counts, void* workspace,
+                         int64_t workspace_bytes, int* status, void* stream);
+int dsv4_balance_backward(const void* logits, int32_t dtype, int64_t n_tokens, int32_t n_experts, int32_t n_seqs,
+                          int32_t score_func, float alpha, const float* grad_loss, void* dlogits,
+                          const void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ *
  * Router: OffloadDeepseekV4MoE._route (deepseek_v4.py:118-148).
  * logits = float(x) @ gate_w^T; scores by score_func; experts = top-k of
  * scores + bias (or tid2eid[input_ids] when tid2eid != NULL, the table
