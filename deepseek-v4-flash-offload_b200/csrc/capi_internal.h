@@ -23,12 +23,12 @@ int bind_device_of(const void* ptr, int* device);
 // caller's device again (for entry points called from code that keeps its own
 // current device).
 struct DeviceScope {
-  int prev = -1;
+  int prev = -1, device = -1;
   int enter(const void* ptr) {
-    int cur = -1, dev = -1;
+    int cur = -1;
     if (cudaGetDevice(&cur) != cudaSuccess) cur = -1;
-    if (int rc = bind_device_of(ptr, &dev)) return rc;
-    if (cur >= 0 && cur != dev) prev = cur;
+    if (int rc = bind_device_of(ptr, &device)) return rc;
+    if (cur >= 0 && cur != device) prev = cur;
     return DSV4_OK;
   }
   ~DeviceScope() {

@@ -8,15 +8,21 @@
 // read either major order from shared memory, so the gradient of a linear
 // layer's input uses the same stored weight.
 //
-// Weights are the M side of the MMA (128 of N per CTA), tokens its N side (BN
-// of M, 16 to 128), so that one token still feeds whole 128-row MMAs.
 // E8M0 scales: tcgen05 kind::mxf8f6f4 applies them.  Its four scale bytes per
 //   row (32 of K each) hold the scales of four consecutive 128-blocks instead,
 //   and the four MMAs of a k-tile all name byte (kt % 4): one 4-byte word per
 //   row and 512 of K, the bytes as they lie in memory.
 // fp32 scales: kind::f8f6f4 into a ring of TMEM accumulators, one k-tile each;
 //   the epilogue warps add as * bs times each partial sum to fp32 registers.
+//   Handing an accumulator over (commit, load, release) takes about as long as
+//   three k-tiles' MMAs, hence four of them.
+//
+// Two kernels share the roles (TMA producer, MMA issuer, scale loader,
+// epilogue): a CTA per 128 of N and up to 128 rows of a whose K a cluster
+// splits (few rows: latency, HBM), and a persistent one of CTA pairs (many
+// rows: tensor cores, L2).  fp8_shape() chooses.
 #include <algorithm>
+#include <atomic>
 
 #include "capi_internal.h"
 #include "common.cuh"
@@ -33,6 +39,21 @@ constexpr int F_EPI_WARP0 = 4;
 // Set by a kernel whose bounded wait ran out; read by dsv4_fp8_status.
 __device__ int g_fp8_status;
 
+struct Fp8Params {
+  const void* as;      // [M, kb] bytes or floats
+  const void* bs;      // element (kb, nb) at kb * bs_k + nb * bs_n
+  int64_t bs_k, bs_n;
+  void* y;
+  int64_t ldy, M, N;
+  int kb;              // scale blocks along K = k-tiles
+  int vec;             // access width of a row of `as` (scale_vec)
+  int out_f32;         // y is fp32, else bf16
+  int vec_y;           // rows of y take vector stores
+};
+
+// ---------------------------------------------------------------------------
+// waits, cluster and issue helpers
+// ---------------------------------------------------------------------------
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -44,28 +65,43 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0u;
 }
-// Bounded wait on a barrier that CTAs of the cluster may arrive on.  The clock
-// is read once in 1024 tries, since reading %globaltimer costs more than the
-// k-tile a role waits for.  False once a wait of this CTA has run out.
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, int* status) {
+// Bounded wait of a whole warp; every lane gets the same answer.  False once a
+// wait of this CTA has run out.  CLUSTER: what another CTA wrote before its
+// arrival is read after the wait (the fence that this takes is not free).
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status) {
   uint64_t t0 = 0;
+  bool ok = true;
   for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if (i % 64 == 0 && read_status(status) == DSV4_ETIMEOUT) return false;
+    if (CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) break;
+    if (i % 64 == 0 && read_status(status) == DSV4_ETIMEOUT) {
+      ok = false;
+      break;
+    }
     if (i % 1024 == 0) {
       const uint64_t now = globaltimer_ns();
       if (t0 == 0) t0 = now;
       else if (now - t0 > DSV4_WAIT_NS) {
         set_status(status, DSV4_ETIMEOUT);
-        return false;
+        ok = false;
+        break;
       }
     }
   }
+  return __all_sync(0xffffffffu, ok);
 }
-
-// bar_wait of a whole warp: every lane gets the same answer.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* status) {
-  return __all_sync(0xffffffffu, bar_wait(bar, parity, status));
+// Whether the phase has completed, for a later `__all_sync(~0u, ...) ||
+// warp_wait(...)`: a look ahead whose latency hides behind other work.
+__device__ __forceinline__ uint32_t bar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
 }
 // One lane of a converged warp, always the same one.  The roles that issue TMA
 // and tcgen05 operations run warp-uniformly and elect a lane for the issue:
@@ -79,35 +115,40 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(p));
   return p != 0u;
 }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Address of this CTA's shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Arrival that publishes nothing (an accumulator has been read: its values are
+// in registers).  A release at cluster scope here cost 0.6 us per k-tile.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
 
-struct Fp8Params {
-  const void* as;      // [M, kb] bytes or floats
-  const void* bs;      // element (kb, nb) at kb * bs_k + nb * bs_n
-  int64_t bs_k, bs_n;
-  void* y;
-  int64_t ldy, M, N;
-  int kb;              // scale blocks along K = k-tiles
-  int vec;             // access width of a row of `as` (scale_vec)
-};
-
-template <int BN, bool E8>
-struct FCfg {
-  static constexpr int A_BYTES = F_BM * F_BK;
-  static constexpr int B_BYTES = BN * F_BK;
-  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  // two CTAs share an SM: their rings stay within half of its shared memory
-  static constexpr int STAGES = BN == 128 ? 3 : (BN == 64 ? 4 : 5);
-  static constexpr int SLOT_BYTES = E8 ? 1024 : F_GROUP * BN * 4;
-  static constexpr int EPI_WARPS = BN == 128 ? 8 : 4;
-  static constexpr int COLS = BN / (EPI_WARPS / 4);      // accumulator columns per epilogue warp
-  static constexpr int THREADS = (F_EPI_WARP0 + EPI_WARPS) * 32;
-  static constexpr int NACC = E8 ? 1 : (BN == 128 ? 2 : 4);
-  static constexpr int SF_COL = BN;                      // E8M0: 8 columns of scales, twice
-  static constexpr uint32_t TMEM_COLS = E8 ? (BN == 128 ? 256 : (BN == 64 ? 128 : (BN == 32 ? 64 : 32))) : NACC * BN;
-  static constexpr int BARS = 2 * STAGES + 2 * F_SLOTS + 2 * NACC + 1;
-  static constexpr int SMEM = STAGES * STAGE_BYTES + F_SLOTS * SLOT_BYTES + BARS * 8 + 16 + 1024;
-};
-
+// ---------------------------------------------------------------------------
+// tcgen05
+// ---------------------------------------------------------------------------
 __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                           uint32_t accumulate) {
   asm volatile(
@@ -117,27 +158,71 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t adesc, uint6
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Instruction descriptor of kind::f8f6f4 with E4M3 A and B, fp32 D.
-__host__ __device__ __forceinline__ uint32_t idesc_f8(int m, int n) {
+__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_mxf8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t accumulate, uint32_t sfa_tmem, uint32_t sfb_tmem) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
+      : "memory");
+}
+__device__ __forceinline__ void tc_cp_sf_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// Arrival on the same barrier of both CTAs once the MMAs issued so far are done.
+__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+// Instruction descriptors: kind::f8f6f4 with E4M3 A and B, fp32 D; either
+// kind's bits for an operand stored along M / N; kind::mxf8f6f4 with M = 256.
+__device__ __forceinline__ uint32_t idesc_f8(int m, int n) {
   return (1u << 4) | (((uint32_t)(n >> 3) & 63u) << 17) | (((uint32_t)(m >> 4) & 31u) << 24);
 }
-constexpr uint32_t IDESC_A_MN = 1u << 15;   // operand A stored along M (both kinds)
+constexpr uint32_t IDESC_A_MN = 1u << 15;
+constexpr uint32_t IDESC_B_MN = 1u << 16;
+__device__ __forceinline__ uint32_t idesc_mxf8_pair(int n, uint32_t sf_id) {
+  return (idesc_mxf8f6f4(n, false, sf_id, true) & ~(31u << 24)) | ((256u >> 4) << 24);
+}
+// Into this CTA's shared memory, the bytes counted by a barrier of the pair.
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
+                                                 uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "l"(policy)
+      : "memory");
+}
 
-// Scales of F_CHUNK k-tiles at a time.  Rows of `as` are loaded with the widest
-// access that their start allows, and the loads of a chunk are all in flight
-// together (one byte-wise load per k-tile kept the tensor cores waiting: 0.8 us
-// a k-tile instead of 0.3).  Read past L1: the kernel just before may have
-// written them.  Past the end of K: byte 127 (= 1) or float 0; the operand
-// bytes there are zero.
-constexpr int F_CHUNK = 16;
+// ---------------------------------------------------------------------------
+// Scales of 16 (E8M0) or 4 (fp32) k-tiles at a time, a chunk ahead of their
+// use.  Rows of `as` are loaded with the widest access that their start
+// allows, and the loads of a chunk are all in flight together (one byte-wise
+// load per k-tile kept the tensor cores waiting: 0.8 us a k-tile instead of
+// 0.28).  Read past L1: the kernel just before may have written them.  Past
+// the end of K: byte 127 (= 1) or float 0; the operand bytes there are zero.
+// ---------------------------------------------------------------------------
 // Access width of the rows of `as`, in elements: 16, 4 or 1 bytes, 4 or 1 floats.
-__host__ __device__ __forceinline__ int scale_vec(const void* as, int kb, bool e8) {
+inline int scale_vec(const void* as, int kb, bool e8) {
   if (!e8) return kb % 4 == 0 && (uintptr_t)as % 16 == 0 ? 4 : 1;
   return kb % 16 == 0 && (uintptr_t)as % 16 == 0 ? 16 : (kb % 4 == 0 && (uintptr_t)as % 4 == 0 ? 4 : 1);
 }
 // Words w[g] = bytes of k-tiles kt + 4 g ..+ 3 of the row at p.
-__device__ __forceinline__ void sf_row(const uint8_t* p, int kt, int kb, int vec, bool in, uint32_t w[4]) {
-  if (in && vec == 16) {   // kb % 16 == 0: a chunk never runs past the end
+__device__ __forceinline__ void sf_row(const uint8_t* p, int kt, int kb, int vec, bool in, uint32_t (&w)[4]) {
+  if (in && vec == 16) {   // rows are multiples of 16 bytes: a chunk never leaves its row
     const uint4 v = __ldcg(reinterpret_cast<const uint4*>(p + kt));
     w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     return;
@@ -156,7 +241,7 @@ __device__ __forceinline__ void sf_row(const uint8_t* p, int kt, int kb, int vec
     }
   }
 }
-// The byte of one of 32 k-tiles from kt, a lane each (a block column of bs).
+// The byte of k-tile kt of a block column, a lane each of 32.
 __device__ __forceinline__ uint32_t sf_lane(const uint8_t* p, int64_t stride, int kt, int kb, bool in) {
   return in && kt < kb ? (uint32_t)__ldcg(p + (int64_t)kt * stride) : 127u;
 }
@@ -167,26 +252,55 @@ __device__ __forceinline__ uint32_t sf_gather(uint32_t b, int l0) {
   for (int i = 0; i < 4; ++i) w |= __shfl_sync(0xffffffffu, b, l0 + i) << (8 * i);
   return w;
 }
-// f[i] = float of k-tile kt + i of the row at p, N a multiple of 4.
-template <int N>
-__device__ __forceinline__ void scale_row(const float* p, int kt, int kb, int vec, bool in, float f[N]) {
+// f[i] = float of k-tile kt + i of the row at p.
+__device__ __forceinline__ void scale_row(const float* p, int kt, int kb, int vec, bool in, float (&f)[F_GROUP]) {
+  if (vec == 4) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in && kt < kb) v = __ldcg(reinterpret_cast<const float4*>(p + kt));
+    f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
+  } else {
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    if (vec == 4) {
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (in && kt + i < kb) v = __ldcg(reinterpret_cast<const float4*>(p + kt + i));
-      f[i] = v.x, f[i + 1] = v.y, f[i + 2] = v.z, f[i + 3] = v.w;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[i + j] = in && kt + i + j < kb ? __ldcg(p + kt + i + j) : 0.f;
-    }
+    for (int j = 0; j < F_GROUP; ++j) f[j] = in && kt + j < kb ? __ldcg(p + kt + j) : 0.f;
   }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows: weights are the M side of the MMA (128 of N per CTA), rows of a
+// its N side (BN), so that one row still feeds whole 128-row MMAs.  The CTAs
+// of a cluster take a share of K each; at the end every CTA adds one slice of
+// the tile over the others' shared memory, in rank order.
+//   warp 0: TMA producer, warp 1: MMA issuer, warp 2: scales, warp 3: TMEM
+//   warps 4..: epilogue, 32 of N each (lane = weight row, columns = rows of a)
+// ---------------------------------------------------------------------------
+template <int BN, bool E8>
+struct FCfg {
+  static constexpr int A_BYTES = F_BM * F_BK;
+  static constexpr int B_BYTES = BN * F_BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  // Two CTAs share an SM: their rings stay within half of its shared memory.
+  static constexpr int STAGES = BN == 128 ? (E8 ? 3 : 4) : (BN == 64 ? 4 : 5);
+  static constexpr int SLOT_BYTES = E8 ? 1024 : F_GROUP * BN * 4;
+  static constexpr int EPI_WARPS = BN >= 64 ? 8 : 4;
+  static constexpr int COLS = BN / (EPI_WARPS / 4);      // accumulator columns per epilogue warp
+  static constexpr int THREADS = (F_EPI_WARP0 + EPI_WARPS) * 32;
+  static constexpr int NACC = E8 ? 1 : 4;
+  static constexpr int SF_COL = BN;                      // E8M0: 8 columns of scales, twice
+  static constexpr uint32_t TMEM_COLS = E8 ? (BN == 128 ? 256 : (BN == 64 ? 128 : (BN == 32 ? 64 : 32))) : NACC * BN;
+  static constexpr int BARS = 2 * STAGES + 2 * F_SLOTS + 2 * NACC + 1;
+  static constexpr int RED_BYTES = BN * F_BM * 4;        // fp32 results, in the ring after the last MMA
+  static constexpr int SMEM = STAGES * STAGE_BYTES + F_SLOTS * SLOT_BYTES + BARS * 8 + 16 + 1024;
+  static_assert(RED_BYTES <= STAGES * STAGE_BYTES, "the ring holds the results");
+  // The CTAs of a cluster wait for one another, so a CTA that is resident must
+  // get its TMEM without waiting for another resident one: at most two of
+  // these CTAs fit an SM (shared memory), and either both take at most half
+  // of the 512 columns or one leaves no room for the other.
+  static_assert(SMEM > 76 * 1024 && (TMEM_COLS <= 256 || SMEM > 134 * 1024), "two CTAs share an SM's TMEM");
+};
+
 template <int BN, bool E8, bool A_MN>
-__global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
+__global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                      const Fp8Params p, const int out_f32) {
+                      const Fp8Params p, const int per) {
   using C = FCfg<BN, E8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -203,7 +317,9 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp-uniform
   const int n0 = blockIdx.x * F_BM;
   const int64_t m0 = (int64_t)blockIdx.y * BN;
-  const int nkt = p.kb;
+  // this CTA's k-tiles: kbeg .. kbeg + nkt - 1 (`per`, a multiple of 4, per CTA of the cluster)
+  const int split = gridDim.z, rank = blockIdx.z;
+  const int kbeg = rank * per, nkt = min(per, p.kb - kbeg);
   const int ngr = (nkt + F_GROUP - 1) / F_GROUP;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -243,11 +359,12 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
       const int s = kt % C::STAGES;
       if (kt >= C::STAGES && !warp_wait(&empty[s], (uint32_t)(kt / C::STAGES - 1) & 1u, err)) break;
       uint8_t* st = smem + s * C::STAGE_BYTES;
+      const int k0 = (kbeg + kt) * F_BK;
       if (elect_one()) {
         mbar_expect_tx(&full[s], C::STAGE_BYTES);
-        if constexpr (A_MN) tma_load_2d(st, &tmW, &full[s], n0, kt * F_BK, pol);
-        else tma_load_2d(st, &tmW, &full[s], kt * F_BK, n0, pol);
-        tma_load_2d(st + C::A_BYTES, &tmX, &full[s], kt * F_BK, (int)m0, pol);
+        if constexpr (A_MN) tma_load_2d(st, &tmW, &full[s], n0, k0, pol);
+        else tma_load_2d(st, &tmW, &full[s], k0, n0, pol);
+        tma_load_2d(st + C::A_BYTES, &tmX, &full[s], k0, (int)m0, pol);
         mbar_arrive(&full[s]);
       }
       __syncwarp();
@@ -300,8 +417,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             tc_mma_f8(tmem + ab * BN, dA + A_STEP * j, dB + 2u * j, idesc, j != 0 ? 1u : 0u);
-          tc_commit(&empty[s]);
-          tc_commit(&accfull[ab]);
+          tc_commit(&empty[s]);   // the stage is free and the accumulator is full
         }
       }
       __syncwarp();
@@ -318,19 +434,20 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
     __syncwarp();
   } else if (warp == 2) {
     // ---------------------------------------------------------------- scales
-    constexpr int ROWS = (BN + 31) / 32;   // token rows per lane
+    constexpr int ROWS = (BN + 31) / 32;                       // rows of a per lane
+    const int vec = kbeg % 16 == 0 ? p.vec : min(p.vec, 4);
     if constexpr (E8) {
-      const uint8_t* bs = static_cast<const uint8_t*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n;
+      const uint8_t* bs = static_cast<const uint8_t*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n + (int64_t)kbeg * p.bs_k;
       uint32_t cur[ROWS][4], nxt[ROWS][4], wbyte = 0;
-      auto load = [&](int kt, uint32_t (&w)[ROWS][4]) {
+      auto load = [&](int kt) {
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
           const int64_t m = m0 + lane + 32 * j;
           const bool in = lane + 32 * j < BN && m < p.M;
-          sf_row(static_cast<const uint8_t*>(p.as) + (in ? m * nkt : 0), kt, nkt, p.vec, in, w[j]);
+          sf_row(static_cast<const uint8_t*>(p.as) + (in ? m * p.kb + kbeg : 0), kt, nkt, vec, in, nxt[j]);
         }
       };
-      load(0, nxt);
+      load(0);
       bool ok = true;
       for (int gr = 0; gr < ngr && ok; gr += 4) {
         if (gr % 8 == 0) wbyte = sf_lane(bs, p.bs_k, gr * F_GROUP + lane, nkt, true);
@@ -338,7 +455,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
         for (int j = 0; j < ROWS; ++j)
 #pragma unroll
           for (int g = 0; g < 4; ++g) cur[j][g] = nxt[j][g];
-        if (gr + 4 < ngr) load((gr + 4) * F_GROUP, nxt);
+        if (gr + 4 < ngr) load((gr + 4) * F_GROUP);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           if (gr + g >= ngr) break;
@@ -357,17 +474,17 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
         }
       }
     } else {
-      const float* bs = static_cast<const float*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n;
+      const float* bs = static_cast<const float*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n + (int64_t)kbeg * p.bs_k;
       float cur[ROWS][F_GROUP], nxt[ROWS][F_GROUP], sb = 0.f;
-      auto load = [&](int kt, float (&f)[ROWS][F_GROUP]) {
+      auto load = [&](int kt) {
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
           const int64_t m = m0 + lane + 32 * j;
           const bool in = lane + 32 * j < BN && m < p.M;
-          scale_row<F_GROUP>(static_cast<const float*>(p.as) + (in ? m * nkt : 0), kt, nkt, p.vec, in, f[j]);
+          scale_row(static_cast<const float*>(p.as) + (in ? m * p.kb + kbeg : 0), kt, nkt, vec, in, nxt[j]);
         }
       };
-      load(0, nxt);
+      load(0);
       for (int gr = 0; gr < ngr; ++gr) {
         const int slot = gr % F_SLOTS, kt0 = gr * F_GROUP;
         if (gr % 8 == 0) sb = kt0 + lane < nkt ? __ldcg(bs + (int64_t)(kt0 + lane) * p.bs_k) : 0.f;
@@ -375,7 +492,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
         for (int j = 0; j < ROWS; ++j)
 #pragma unroll
           for (int i = 0; i < F_GROUP; ++i) cur[j][i] = nxt[j][i];
-        if (gr + 1 < ngr) load(kt0 + F_GROUP, nxt);
+        if (gr + 1 < ngr) load(kt0 + F_GROUP);
         if (gr >= F_SLOTS && !warp_wait(&sempty[slot], (uint32_t)(gr / F_SLOTS - 1) & 1u, err)) break;
         float* f = reinterpret_cast<float*>(slots + slot * C::SLOT_BYTES);
 #pragma unroll
@@ -393,62 +510,98 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
     // -------------------------------------------------------------- epilogue
     const int q = warp & 3, c0 = ((warp - F_EPI_WARP0) >> 2) * C::COLS;
     const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
-    float acc[C::COLS];
-    bool ok = true;
+    float* red = reinterpret_cast<float*>(smem) + c0 * F_BM + q * 32 + lane;   // [row of a][128 of N]
     if constexpr (E8) {
-      ok = __all_sync(0xffffffffu, bar_wait(&accfull[0], 0, err) && read_status(err) == 0);
-      tc_fence_after();
-      if (ok) {
-#pragma unroll
-        for (int c = 0; c < C::COLS; c += 16) tmem_ld16(trow + c, acc + c);
-        tc_wait_ld();
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < C::COLS; ++c) acc[c] = 0.f;
-      for (int kt = 0; kt < nkt; ++kt) {
-        const int ab = kt % C::NACC, gr = kt / F_GROUP, slot = gr % F_SLOTS;
-        const bool mine = (kt % F_GROUP != 0 || bar_wait(&sfull[slot], (uint32_t)(gr / F_SLOTS) & 1u, err)) &&
-                          bar_wait(&accfull[ab], (uint32_t)(kt / C::NACC) & 1u, err);
-        if (!(ok = __all_sync(0xffffffffu, mine))) break;
+      if (warp_wait(&accfull[0], 0, err)) {
         tc_fence_after();
-        const float* f = reinterpret_cast<const float*>(slots + slot * C::SLOT_BYTES) + (kt % F_GROUP) * BN + c0;
 #pragma unroll
         for (int c = 0; c < C::COLS; c += 16) {
           float v[16];
-          tmem_ld16(trow + ab * BN + c, v);
+          tmem_ld16(trow + c, v);
           tc_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; j += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(f + c + j);
-            acc[c + j] = fmaf(v[j], s.x, acc[c + j]);
-            acc[c + j + 1] = fmaf(v[j + 1], s.y, acc[c + j + 1]);
-            acc[c + j + 2] = fmaf(v[j + 2], s.z, acc[c + j + 2]);
-            acc[c + j + 3] = fmaf(v[j + 3], s.w, acc[c + j + 3]);
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&accempty[ab]);
-          if (kt % F_GROUP == F_GROUP - 1 || kt == nkt - 1) mbar_arrive(&sempty[slot]);
+          for (int j = 0; j < 16; ++j) red[(c + j) * F_BM] = v[j];
         }
       }
-    }
-    const int64_t n = (int64_t)n0 + q * 32 + lane;
-    if (ok && n < p.N) {
+    } else {
+      float acc[C::COLS];
 #pragma unroll
-      for (int c = 0; c < C::COLS; ++c) {
-        const int64_t m = m0 + c0 + c;
-        if (m < p.M) {
-          if (out_f32) static_cast<float*>(p.y)[m * p.ldy + n] = acc[c];
-          else static_cast<uint16_t*>(p.y)[m * p.ldy + n] = bf16_bits(acc[c]);
+      for (int c = 0; c < C::COLS; ++c) acc[c] = 0.f;
+      bool ok = true;
+      for (int kt = 0; kt < nkt; ++kt) {
+        const int ab = kt % C::NACC, gr = kt / F_GROUP, slot = gr % F_SLOTS;
+        if (kt % F_GROUP == 0 && !(ok = warp_wait(&sfull[slot], (uint32_t)(gr / F_SLOTS) & 1u, err))) break;
+        if (!(ok = warp_wait(&empty[kt % C::STAGES], (uint32_t)(kt / C::STAGES) & 1u, err))) break;
+        tc_fence_after();
+        float v[C::COLS];
+#pragma unroll
+        for (int c = 0; c < C::COLS; c += 16) tmem_ld16(trow + ab * BN + c, v + c);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&accempty[ab]);
+        const float* f = reinterpret_cast<const float*>(slots + slot * C::SLOT_BYTES) + (kt % F_GROUP) * BN + c0;
+#pragma unroll
+        for (int c = 0; c < C::COLS; c += 4) {
+          const float4 s = *reinterpret_cast<const float4*>(f + c);
+          acc[c] = fmaf(v[c], s.x, acc[c]);
+          acc[c + 1] = fmaf(v[c + 1], s.y, acc[c + 1]);
+          acc[c + 2] = fmaf(v[c + 2], s.z, acc[c + 2]);
+          acc[c + 3] = fmaf(v[c + 3], s.w, acc[c + 3]);
         }
+        __syncwarp();
+        if (lane == 0 && (kt % F_GROUP == F_GROUP - 1 || kt == nkt - 1)) mbar_arrive(&sempty[slot]);
+      }
+      // the last accumulator is full: no MMA reads the ring any more
+      if (ok) {
+#pragma unroll
+        for (int c = 0; c < C::COLS; ++c) red[c * F_BM] = acc[c];
       }
     }
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  // the cluster's partial results, each CTA a slice, added in rank order
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+  const int rows = (int)min((int64_t)BN, p.M - m0), units = rows * (F_BM / 4);   // of four columns
+  const int u1 = (int)((int64_t)units * (rank + 1) / split);
+  for (int u = (int)((int64_t)units * rank / split) + (int)threadIdx.x; u < u1; u += C::THREADS) {
+    const float* src = reinterpret_cast<const float*>(smem) + u * 4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (split == 1) {
+      a = *reinterpret_cast<const float4*>(src);
+    } else {
+      for (int r = 0; r < split; ++r) {
+        const float4 v = ld_cluster_f4(map_rank(src, r));
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+      }
+    }
+    const int64_t n = (int64_t)n0 + u % (F_BM / 4) * 4, at = (m0 + u / (F_BM / 4)) * p.ldy + n;
+    const float o[4] = {a.x, a.y, a.z, a.w};
+    if (p.out_f32) {
+      float* y = static_cast<float*>(p.y) + at;
+      if (p.vec_y && n + 4 <= p.N) {
+        *reinterpret_cast<float4*>(y) = a;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) y[j] = o[j];
+      }
+    } else {
+      uint16_t* y = static_cast<uint16_t*>(p.y) + at;
+      if (p.vec_y && n + 4 <= p.N) {
+        *reinterpret_cast<uint2*>(y) = make_uint2(bf16_bits(a.x) | ((uint32_t)bf16_bits(a.y) << 16),
+                                                  bf16_bits(a.z) | ((uint32_t)bf16_bits(a.w) << 16));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.N) y[j] = bf16_bits(o[j]);
+      }
+    }
+  }
+  __syncwarp();
+  if (split > 1) cluster_sync();   // the others have read this CTA's part
   if (threadIdx.x == 0 && *err) set_status(&g_fp8_status, *err);
   if (warp == 3) {
     tc_fence_after();
@@ -456,109 +609,51 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, 1)
   }
 }
 
-template <int BN, bool E8, bool A_MN>
-int launch_small(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int out_f32, cudaStream_t st) {
-  using C = FCfg<BN, E8>;
-  auto k = fp8_matmul_kernel<BN, E8, A_MN>;
-  DSV4_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-  const dim3 grid((unsigned)((p.N + F_BM - 1) / F_BM), (unsigned)((p.M + BN - 1) / BN));
-  DSV4_CUDA_CHECK(launch_k(k, grid, dim3(C::THREADS), C::SMEM, st, pdl_enabled(), tw, tx, p, out_f32));
-  return DSV4_OK;
-}
-
-template <int BN>
-int launch_small_v(bool e8, bool a_mn, const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int out_f32,
-                   cudaStream_t st) {
-  if (e8) return a_mn ? launch_small<BN, true, true>(tw, tx, p, out_f32, st) : launch_small<BN, true, false>(tw, tx, p, out_f32, st);
-  return a_mn ? launch_small<BN, false, true>(tw, tx, p, out_f32, st) : launch_small<BN, false, false>(tw, tx, p, out_f32, st);
-}
-
-
 // ---------------------------------------------------------------------------
-// Large products: CTA pairs.  Tokens are the M side (128 rows per CTA, 256 per
-// pair), weights the N side (256, half of them in each CTA's shared memory):
-// tcgen05.mma.cta_group::2 reads both halves, so a CTA loads 32 KB per k-tile
-// for 128 x 256 x 128 products and the pair's tile has half the operand
-// traffic of two separate 128 x 256 tiles.  Persistent: one pair per two SMs
-// walks the tiles, with the ring running ahead into the next tile.
+// Many rows: CTA pairs.  Rows of a are the M side (128 per CTA, 256 per pair),
+// weights the N side, half of them in each CTA's shared memory:
+// tcgen05.mma.cta_group::2 reads both halves, so the pair's tile has half the
+// operand traffic of two separate ones.  Persistent: one pair per two SMs
+// walks the tiles, the ring running ahead into the next tile.
 //   warp 0: TMA producer (each CTA its own halves, into the leader's barrier)
-//   warp 1: MMA issuer (leader CTA only)
-//   warp 2: E8M0 scale words (tokens' rows of this CTA, the weights' blocks)
+//   warp 1: MMA issuer (leader CTA), or passing free accumulators on to it
+//   warp 2: scales (the rows of this CTA, the weights' blocks)
 //   warps 4-11: epilogue, 32 rows x 128 columns each
-// E8M0: one 256-column accumulator, released as soon as the epilogue has it in
-// registers.  fp32 scales: two accumulators, a k-tile each; an epilogue thread
-// holds one row of one 128-block, so a partial sum takes one multiply-add.
+// E8M0: one accumulator of 256 columns, released as soon as the epilogue has it
+// in registers.  fp32 scales: two of 256 columns, a k-tile each; an epilogue
+// thread has one row of one 128-block of N, so a partial sum takes one
+// multiply-add.  (Four accumulators of 128 columns would hide the hand-over
+// better, but MMAs of 128 columns read a's tile from shared memory twice as
+// often, and that bandwidth is the limit: 1.24 us per k-tile of 256 x 256.)
 // ---------------------------------------------------------------------------
-constexpr int L_TM = 256, L_TN = 256;
-constexpr int L_STAGES = 6;
-constexpr int L_STAGE_BYTES = 2 * 128 * F_BK;
-constexpr int L_SLOT_BYTES = 3 * 512;            // scale atoms: 128 rows of a, two blocks of b
+constexpr int L_TM = 256;
 constexpr int L_SF_COL = 256;                    // 12 columns of scales, twice
-constexpr int L_EPI_WARPS = 8;
-constexpr int L_THREADS = (F_EPI_WARP0 + L_EPI_WARPS) * 32;
 constexpr int L_RASTER = 8;                      // m-tiles walked together: their operands meet in L2
-constexpr int L_SMEM = L_STAGES * L_STAGE_BYTES + F_SLOTS * L_SLOT_BYTES + 512 + 1024;
+constexpr int L_OUT_BYTES = 32 * 128;            // per epilogue warp: 32 rows x 128 bytes
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Address of this CTA's shared variable in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  return a;
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
-}
-// Into this CTA's shared memory, the bytes counted by a barrier of the pair.
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
-                                                 uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4}], [%2], %5;" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(bar), "r"(c0), "r"(c1), "l"(policy)
-      : "memory");
-}
-// Arrival on the same barrier of both CTAs once the MMAs issued so far are done.
-__device__ __forceinline__ void tc_commit_pair(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-          smem_u32(bar)),
-      "h"((uint16_t)3)
-      : "memory");
-}
-__device__ __forceinline__ void tc_cp_sf_pair(uint32_t taddr, uint64_t sdesc) {
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
-}
-__device__ __forceinline__ void tc_mma_f8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                               uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void tc_mma_mxf8_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                                 uint32_t accumulate, uint32_t sfa_tmem, uint32_t sfb_tmem) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}\n" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(sfa_tmem), "r"(sfb_tmem)
-      : "memory");
-}
-constexpr uint32_t IDESC_B_MN = 1u << 16;   // operand B stored along N
-// kind::mxf8f6f4 descriptor (E4M3 both) with M = 256 instead of 128.
-__device__ __forceinline__ uint32_t idesc_mxf8_pair(uint32_t sf_id) {
-  return (idesc_mxf8f6f4(L_TN, false, sf_id, true) & ~(31u << 24)) | ((256u >> 4) << 24);
-}
+constexpr int L_TN = 256;
+constexpr int L_A_BYTES = 128 * F_BK;
+constexpr int L_STAGE_BYTES = L_A_BYTES + L_TN / 2 * F_BK;
+
+template <bool E8>
+struct LCfg {
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int COLS = L_TN / (EPI_WARPS / 4);       // accumulator columns per epilogue warp
+  static constexpr int THREADS = (F_EPI_WARP0 + EPI_WARPS) * 32;
+  static constexpr int NACC = E8 ? 1 : 2;
+  static constexpr int STAGES = 5;
+  // E8M0: scale atoms of 128 rows of a and two blocks of b; fp32: as * bs of
+  // four k-tiles, two blocks of N and 128 rows
+  static constexpr int SLOT_BYTES = E8 ? 3 * 512 : F_GROUP * 2 * 128 * 4;
+  static constexpr int BARS = 2 * STAGES + 2 * F_SLOTS + 2 * NACC + 1;
+  static constexpr int SMEM =
+      STAGES * L_STAGE_BYTES + EPI_WARPS * L_OUT_BYTES + F_SLOTS * SLOT_BYTES + BARS * 8 + 16 + 1024;
+  // fp32: the four issuing warps give registers to the epilogue (128 sums and
+  // 64 values on their way from TMEM per thread); the shares add up to no more
+  // than the block is launched with
+  static constexpr int REGS_ISSUE = 56, REGS_EPI = 224, REGS_LAUNCH = 168;
+  static_assert(REGS_ISSUE * 128 + REGS_EPI * EPI_WARPS * 32 <= REGS_LAUNCH * THREADS, "register split");
+};
 
 struct LTile {
   int64_t m0;
@@ -573,55 +668,74 @@ __device__ __forceinline__ LTile large_tile(int t, int mt, int nt) {
   return o;
 }
 
-// 128 columns of a row from n0, columns >= N left alone; vec: 16-byte stores.
-__device__ __forceinline__ void store_row(const float (&acc)[128], const Fp8Params& p, int64_t m, int64_t n0,
-                                          int out_f32, bool vec) {
-  if (out_f32) {
-    float* y = static_cast<float*>(p.y) + m * p.ldy + n0;
+// The 32 x COLS results of an epilogue warp, a lane per row, to rows m0 .. of y
+// and columns n0 .., 128 bytes of each row at a time through the warp's staging
+// buffer (16-byte units swizzled by row): every store then covers whole
+// 128-byte lines of four rows instead of 16 bytes of 32.
+template <int COLS>
+__device__ __forceinline__ void store_tile(const float (&acc)[COLS], uint8_t* buf, const Fp8Params& p, int64_t m0,
+                                           int64_t n0, int lane) {
+  const int esz = p.out_f32 ? 4 : 2, per = 128 / esz;   // columns per pass
 #pragma unroll
-    for (int c = 0; c < 128; c += 4) {
-      if (vec && n0 + c + 4 <= p.N) {
-        *reinterpret_cast<float4*>(y + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+  for (int pass = 0; pass < COLS / 32; ++pass) {
+    if (pass >= COLS / 64 && !p.out_f32) break;
+    const int64_t nc = n0 + pass * per;
+    if (nc >= p.N) break;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      uint4 o;
+      if (p.out_f32) {
+        const int c = pass * 32 + u * 4;
+        o = make_uint4(__float_as_uint(acc[c]), __float_as_uint(acc[c + 1]), __float_as_uint(acc[c + 2]),
+                       __float_as_uint(acc[c + 3]));
       } else {
+        const int c = pass * 64 % COLS + u * 8;
+        uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (n0 + c + j < p.N) y[c + j] = acc[c + j];
+          w[j] = bf16_bits(acc[c + 2 * j]) | ((uint32_t)bf16_bits(acc[c + 2 * j + 1]) << 16);
+        o = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      *reinterpret_cast<uint4*>(buf + lane * 128 + ((u ^ (lane & 7)) << 4)) = o;
+    }
+    __syncwarp();
+    if (p.vec_y && nc + per <= p.N) {
+      uint8_t* y = static_cast<uint8_t*>(p.y) + nc * esz + (lane & 7) * 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 4 + (lane >> 3);
+        const uint4 o = *reinterpret_cast<const uint4*>(buf + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+        if (m0 + r < p.M) *reinterpret_cast<uint4*>(y + (m0 + r) * p.ldy * esz) = o;
+      }
+    } else {
+      for (int r = 0; r < 32 && m0 + r < p.M; ++r) {
+        for (int c = lane; c < per && nc + c < p.N; c += 32) {
+          const uint8_t* o = buf + r * 128 + (((c * esz >> 4) ^ (r & 7)) << 4) + (c * esz & 15);
+          if (p.out_f32) static_cast<float*>(p.y)[(m0 + r) * p.ldy + nc + c] = *reinterpret_cast<const float*>(o);
+          else static_cast<uint16_t*>(p.y)[(m0 + r) * p.ldy + nc + c] = *reinterpret_cast<const uint16_t*>(o);
+        }
       }
     }
-  } else {
-    uint16_t* y = static_cast<uint16_t*>(p.y) + m * p.ldy + n0;
-#pragma unroll
-    for (int c = 0; c < 128; c += 8) {
-      if (vec && n0 + c + 8 <= p.N) {
-        uint32_t o[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[j] = bf16_bits(acc[c + 2 * j]) | ((uint32_t)bf16_bits(acc[c + 2 * j + 1]) << 16);
-        *reinterpret_cast<uint4*>(y + c) = make_uint4(o[0], o[1], o[2], o[3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (n0 + c + j < p.N) y[c + j] = bf16_bits(acc[c + j]);
-      }
-    }
+    __syncwarp();
   }
 }
 
 template <bool E8, bool B_MN>
-__global__ void __launch_bounds__(L_THREADS, 1)
+__global__ void __launch_bounds__(LCfg<E8>::THREADS, 1)
     fp8_matmul_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
-                           const Fp8Params p, const int mt, const int nt, const int out_f32, const int vec) {
-  constexpr int NACC = E8 ? 1 : 2;
+                           const Fp8Params p, const int mt, const int nt) {
+  using C = LCfg<E8>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* slots = smem + L_STAGES * L_STAGE_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(slots + F_SLOTS * L_SLOT_BYTES);   // leader's: both CTAs' bytes
-  uint64_t* empty = full + L_STAGES;
-  uint64_t* sfull = empty + L_STAGES;       // leader's: one arrival per CTA
+  uint8_t* outs = smem + C::STAGES * L_STAGE_BYTES;
+  uint8_t* slots = outs + C::EPI_WARPS * L_OUT_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(slots + F_SLOTS * C::SLOT_BYTES);   // leader's: both CTAs' bytes
+  uint64_t* empty = full + C::STAGES;
+  uint64_t* sfull = empty + C::STAGES;      // E8M0, leader's: one arrival per CTA
   uint64_t* sempty = sfull + F_SLOTS;
   uint64_t* accfull = sempty + F_SLOTS;
-  uint64_t* accempty = accfull + NACC;      // leader's: the epilogue warps of both CTAs
-  uint64_t* drain = accempty + NACC;
+  uint64_t* accempty = accfull + C::NACC;   // this CTA's epilogue warps; leader's: and the other CTA's warp 1
+  uint64_t* drain = accempty + C::NACC;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain + 1);
   int* err = reinterpret_cast<int*>(tmem_holder + 1);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp-uniform
@@ -629,17 +743,17 @@ __global__ void __launch_bounds__(L_THREADS, 1)
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int nkt = p.kb, ngr = (nkt + F_GROUP - 1) / F_GROUP, tiles = mt * nt;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L_STAGES; ++s) {
+    for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < F_SLOTS; ++s) {
-      mbar_init(&sfull[s], 2);
-      mbar_init(&sempty[s], 1);
+      mbar_init(&sfull[s], E8 ? 2 : 1);
+      mbar_init(&sempty[s], E8 ? 1 : C::EPI_WARPS);
     }
-    for (int s = 0; s < NACC; ++s) {
+    for (int s = 0; s < C::NACC; ++s) {
       mbar_init(&accfull[s], 1);
-      mbar_init(&accempty[s], 2 * L_EPI_WARPS);
+      mbar_init(&accempty[s], C::EPI_WARPS + (rank == 0 ? 1 : 0));
     }
     mbar_init(drain, 1);
     *err = 0;
@@ -661,6 +775,9 @@ __global__ void __launch_bounds__(L_THREADS, 1)
   griddep_wait();
   griddep_launch();
 
+  if constexpr (!E8) {
+    if (warp < F_EPI_WARP0) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_ISSUE));
+  }
   if (warp == 0) {
     const uint64_t pol = policy_evict_normal();
     int it = 0;
@@ -669,15 +786,15 @@ __global__ void __launch_bounds__(L_THREADS, 1)
       const LTile tl = large_tile(t, mt, nt);
       const int m0 = (int)(tl.m0 + rank * 128), n0 = tl.n0 + (int)rank * 128;
       for (int kt = 0; kt < nkt; ++kt, ++it) {
-        const int s = it % L_STAGES;
-        if (it >= L_STAGES && !(ok = warp_wait(&empty[s], (uint32_t)(it / L_STAGES - 1) & 1u, err))) break;
+        const int s = it % C::STAGES;
+        if (it >= C::STAGES && !(ok = warp_wait(&empty[s], (uint32_t)(it / C::STAGES - 1) & 1u, err))) break;
         uint8_t* st = smem + s * L_STAGE_BYTES;
         const uint32_t bar = map_rank(&full[s], 0);
         if (elect_one()) {
           if (rank == 0) mbar_expect_tx(&full[s], 2 * L_STAGE_BYTES);
           tma_load_2d_pair(st, &tmX, bar, kt * F_BK, m0, pol);
-          if constexpr (B_MN) tma_load_2d_pair(st + 128 * F_BK, &tmW, bar, n0, kt * F_BK, pol);
-          else tma_load_2d_pair(st + 128 * F_BK, &tmW, bar, kt * F_BK, n0, pol);
+          if constexpr (B_MN) tma_load_2d_pair(st + L_A_BYTES, &tmW, bar, n0, kt * F_BK, pol);
+          else tma_load_2d_pair(st + L_A_BYTES, &tmW, bar, kt * F_BK, n0, pol);
           if (rank == 0) mbar_arrive(&full[s]);
         }
         __syncwarp();
@@ -693,7 +810,7 @@ __global__ void __launch_bounds__(L_THREADS, 1)
   } else if (warp == 1) {
     if (rank == 0) {
       const uint32_t mn = B_MN ? IDESC_B_MN : 0u;
-      constexpr uint32_t B_STEP = B_MN ? (32 * 128) >> 4 : 2u;
+      constexpr uint32_t B_STEP = B_MN ? (32 * 128) >> 4 : 2u;   // 32 of K: 32 rows of 128 B, or 32 B of a row
       int it = 0, grp = 0, ti = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs, ++ti) {
@@ -701,22 +818,22 @@ __global__ void __launch_bounds__(L_THREADS, 1)
           if (ti > 0 && !(ok = warp_wait(&accempty[0], (uint32_t)(ti - 1) & 1u, err))) break;
         }
         for (int kt = 0; kt < nkt; ++kt, ++it) {
-          const int s = it % L_STAGES;
-          if (!(ok = warp_wait(&full[s], (uint32_t)(it / L_STAGES) & 1u, err))) break;
+          const int s = it % C::STAGES;
+          if (!(ok = warp_wait(&full[s], (uint32_t)(it / C::STAGES) & 1u, err))) break;
           const uint32_t aA = smem_u32(smem + s * L_STAGE_BYTES);
-          const uint64_t dA = desc_sw128(aA), dB = desc_sw128(aA + 128 * F_BK);
+          const uint64_t dA = desc_sw128(aA), dB = desc_sw128(aA + L_A_BYTES);
           if constexpr (E8) {
-            if (kt % F_GROUP == 0 && kt > 0) ++grp;
+            const bool fresh = kt % F_GROUP == 0;
+            if (fresh && kt > 0) ++grp;
             const int slot = grp % F_SLOTS;
             const uint32_t sfa = tmem + L_SF_COL + 16 * (grp & 1), sfb = sfa + 4;
-            const bool fresh = kt % F_GROUP == 0;
-            if (fresh && !(ok = warp_wait(&sfull[slot], (uint32_t)(grp / F_SLOTS) & 1u, err))) break;
+            if (fresh && !(ok = warp_wait<true>(&sfull[slot], (uint32_t)(grp / F_SLOTS) & 1u, err))) break;
             tc_fence_after();
             const uint32_t id = kt % F_GROUP, sel = id << 30;
-            const uint32_t idesc = idesc_mxf8_pair(id) | mn;
+            const uint32_t idesc = idesc_mxf8_pair(L_TN, id) | mn;
             if (elect_one()) {
               if (fresh) {
-                const uint32_t sl = smem_u32(slots + slot * L_SLOT_BYTES);
+                const uint32_t sl = smem_u32(slots + slot * C::SLOT_BYTES);
                 tc_cp_sf_pair(sfa, desc_sf(sl));
                 tc_cp_sf_pair(sfb, desc_sf(sl + 512));
                 tc_cp_sf_pair(sfb + 4, desc_sf(sl + 1024));
@@ -733,13 +850,12 @@ __global__ void __launch_bounds__(L_THREADS, 1)
             const int ab = it & 1;
             if (it >= 2 && !(ok = warp_wait(&accempty[ab], (uint32_t)(it / 2 - 1) & 1u, err))) break;
             tc_fence_after();
-            const uint32_t idesc = idesc_f8(256, L_TN) | mn;
+            const uint32_t idesc = idesc_f8(L_TM, L_TN) | mn;
             if (elect_one()) {
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                tc_mma_f8_pair(tmem + ab * 256, dA + 2u * j, dB + B_STEP * j, idesc, j != 0 ? 1u : 0u);
-              tc_commit_pair(&empty[s]);
-              tc_commit_pair(&accfull[ab]);
+                tc_mma_f8_pair(tmem + ab * L_TN, dA + 2u * j, dB + B_STEP * j, idesc, j != 0 ? 1u : 0u);
+              tc_commit_pair(&empty[s]);   // the stage is free and the accumulator is full
             }
           }
           __syncwarp();
@@ -750,6 +866,16 @@ __global__ void __launch_bounds__(L_THREADS, 1)
       __syncwarp();
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(drain, 0) && globaltimer_ns() - t0 < DSV4_WAIT_NS) {
+      }
+    } else {
+      // passes this CTA's free accumulators on to the leader: the epilogue
+      // warps then only arrive at home (a remote arrival holds its warp up)
+      const int mine = pair < tiles ? (tiles - 1 - pair) / pairs + 1 : 0, uses = E8 ? mine : mine * nkt;
+      for (int u = 0; u < uses; ++u) {
+        const int ab = u % C::NACC;
+        if (!warp_wait(&accempty[ab], (uint32_t)(u / C::NACC) & 1u, err)) break;
+        if (lane == 0) mbar_arrive_cluster_relaxed(map_rank(&accempty[ab], 0));
+        __syncwarp();
       }
     }
     __syncwarp();
@@ -774,7 +900,7 @@ __global__ void __launch_bounds__(L_THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
               wbyte[j] = sf_lane(static_cast<const uint8_t*>(p.bs) + (int64_t)(nb0 + j) * p.bs_n, p.bs_k,
-                                 gr * F_GROUP + lane, nkt, (nb0 + j) * 128 < p.N);
+                                 gr * F_GROUP + lane, nkt, (int64_t)(nb0 + j) * 128 < p.N);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j)
@@ -786,7 +912,7 @@ __global__ void __launch_bounds__(L_THREADS, 1)
           for (int g = 0; g < 4; ++g) {
             if (gr + g >= ngr) break;
             const int slot = grp % F_SLOTS;
-            uint8_t* sl = slots + slot * L_SLOT_BYTES;
+            uint8_t* sl = slots + slot * C::SLOT_BYTES;
             const uint32_t wb0 = sf_gather(wbyte[0], (gr + g) % 8 * 4), wb1 = sf_gather(wbyte[1], (gr + g) % 8 * 4);
             if (grp >= F_SLOTS && !(ok = warp_wait(&sempty[slot], (uint32_t)(grp / F_SLOTS - 1) & 1u, err))) break;
             *reinterpret_cast<uint4*>(sl + lane * 16) = make_uint4(cur[0][g], cur[1][g], cur[2][g], cur[3][g]);
@@ -799,62 +925,108 @@ __global__ void __launch_bounds__(L_THREADS, 1)
           }
         }
       }
+    } else {
+      int grp = 0;
+      bool ok = true;
+      float cur[4][F_GROUP], nxt[4][F_GROUP], sb[2] = {};
+      auto load = [&](int t, int kt) {
+        const int64_t m0 = large_tile(t, mt, nt).m0 + rank * 128;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t m = m0 + lane + 32 * j;
+          scale_row(static_cast<const float*>(p.as) + (m < p.M ? m * nkt : 0), kt, nkt, p.vec, m < p.M, nxt[j]);
+        }
+      };
+      if (pair < tiles) load(pair, 0);
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        const int nb0 = large_tile(t, mt, nt).n0 / 128;
+        for (int gr = 0; gr < ngr; ++gr, ++grp) {
+          const int slot = grp % F_SLOTS, kt0 = gr * F_GROUP;
+          if (gr % 8 == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              sb[h] = (int64_t)(nb0 + h) * 128 < p.N && kt0 + lane < nkt
+                          ? __ldcg(static_cast<const float*>(p.bs) + (int64_t)(kt0 + lane) * p.bs_k +
+                                   (int64_t)(nb0 + h) * p.bs_n)
+                          : 0.f;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < F_GROUP; ++i) cur[j][i] = nxt[j][i];
+          if (gr + 1 < ngr) load(t, kt0 + F_GROUP);
+          else if (t + pairs < tiles) load(t + pairs, 0);
+          if (grp >= F_SLOTS && !(ok = warp_wait(&sempty[slot], (uint32_t)(grp / F_SLOTS - 1) & 1u, err))) break;
+          float* f = reinterpret_cast<float*>(slots + slot * C::SLOT_BYTES) + lane;   // [k-tile][block][row]
+#pragma unroll
+          for (int i = 0; i < F_GROUP; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float s = __shfl_sync(0xffffffffu, sb[h], gr % 8 * 4 + i);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) f[(i * 2 + h) * 128 + 32 * j] = cur[j][i] * s;
+            }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sfull[slot]);
+        }
+      }
     }
   } else if (warp >= F_EPI_WARP0) {
-    const int q = warp & 3, c0 = ((warp - F_EPI_WARP0) >> 2) * 128;
+    if constexpr (!E8) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_EPI));
+    const int q = warp & 3, c0 = ((warp - F_EPI_WARP0) >> 2) * C::COLS;
     const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c0;
-    int it = 0, ti = 0;
+    uint8_t* buf = outs + (warp - F_EPI_WARP0) * L_OUT_BYTES;
+    int it = 0, ti = 0, grp = 0;
     bool ok = true;
     for (int t = pair; t < tiles && ok; t += pairs, ++ti) {
       const LTile tl = large_tile(t, mt, nt);
-      const int64_t m = tl.m0 + rank * 128 + q * 32 + lane, n0 = tl.n0 + c0;
-      float acc[128];
+      const int64_t m0 = tl.m0 + rank * 128 + q * 32, n0 = tl.n0 + c0;
+      float acc[C::COLS];
       if constexpr (E8) {
-        ok = warp_wait(&accfull[0], (uint32_t)ti & 1u, err);
-        if (!ok) break;
+        if (!(ok = warp_wait(&accfull[0], (uint32_t)ti & 1u, err))) break;
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 128; c += 16) tmem_ld16(trow + c, acc + c);
+        for (int c = 0; c < C::COLS; c += 16) tmem_ld16(trow + c, acc + c);
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_rank(&accempty[0], 0));
+        if (lane == 0) mbar_arrive(&accempty[0]);
       } else {
 #pragma unroll
-        for (int c = 0; c < 128; ++c) acc[c] = 0.f;
-        const bool inm = m < p.M, inn = n0 < p.N;
-        const float* as = static_cast<const float*>(p.as) + (inm ? m * nkt : 0);
-        const float* bs = static_cast<const float*>(p.bs) + (inn ? n0 / 128 * p.bs_n : 0);
-        float sa[F_GROUP], na[F_GROUP], sb = 0.f;
-        scale_row<F_GROUP>(as, 0, nkt, p.vec, inm, na);
+        for (int c = 0; c < C::COLS; ++c) acc[c] = 0.f;
+        bool ready = false;
         for (int kt = 0; kt < nkt; ++kt, ++it) {
-          if (kt % 32 == 0) sb = inn && kt + lane < nkt ? __ldcg(bs + (int64_t)(kt + lane) * p.bs_k) : 0.f;
-          if (kt % F_GROUP == 0) {
-#pragma unroll
-            for (int i = 0; i < F_GROUP; ++i) sa[i] = na[i];
-            if (kt + F_GROUP < nkt) scale_row<F_GROUP>(as, kt + F_GROUP, nkt, p.vec, inm, na);
-          }
-          const float s = sa[0] * __shfl_sync(0xffffffffu, sb, kt % 32);
-          sa[0] = sa[1], sa[1] = sa[2], sa[2] = sa[3];
-          const int ab = it & 1;
-          ok = warp_wait(&accfull[ab], (uint32_t)(it / 2) & 1u, err);
-          if (!ok) break;
+          const int ab = it & 1, slot = grp % F_SLOTS;
+          if (kt % F_GROUP == 0 && !(ok = warp_wait(&sfull[slot], (uint32_t)(grp / F_SLOTS) & 1u, err))) break;
+          const float s = reinterpret_cast<const float*>(
+              slots + slot * C::SLOT_BYTES)[(kt % F_GROUP * 2 + c0 / 128) * 128 + q * 32 + lane];
+          if (!ready && !(ok = warp_wait(&empty[it % C::STAGES], (uint32_t)(it / C::STAGES) & 1u, err))) break;
           tc_fence_after();
+          uint32_t next = 0;
 #pragma unroll
-          for (int c = 0; c < 128; c += 16) {
-            float v[16];
-            tmem_ld16(trow + ab * 256 + c, v);
+          for (int c = 0; c < C::COLS; c += 64) {
+            float v[64];
+#pragma unroll
+            for (int j = 0; j < 64; j += 16) tmem_ld16(trow + (uint32_t)(ab * L_TN + c + j), v + j);
             tc_wait_ld();
+            if (c == C::COLS - 64) {   // the accumulator is in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&accempty[ab]);
+              next = bar_test(&empty[(it + 1) % C::STAGES], (uint32_t)((it + 1) / C::STAGES) & 1u);
+            }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[c + j] = fmaf(v[j], s, acc[c + j]);
+            for (int j = 0; j < 64; ++j) acc[c + j] = fmaf(v[j], s, acc[c + j]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(map_rank(&accempty[ab], 0));
+          ready = __all_sync(0xffffffffu, next != 0u);
+          if (kt % F_GROUP == F_GROUP - 1 || kt == nkt - 1) {
+            if (lane == 0) mbar_arrive(&sempty[slot]);
+            ++grp;
+          }
         }
         if (!ok) break;
       }
-      if (m < p.M) store_row(acc, p, m, n0, out_f32, vec != 0);
+      store_tile(acc, buf, p, m0, n0, lane);
     }
   }
   tc_fence_before();
@@ -867,64 +1039,132 @@ __global__ void __launch_bounds__(L_THREADS, 1)
   }
 }
 
-template <bool E8, bool B_MN>
-int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, int out_f32, int sms,
-                cudaStream_t st) {
-  auto k = fp8_matmul_pair_kernel<E8, B_MN>;
-  DSV4_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, L_SMEM));
-  const int64_t mt = (p.M + L_TM - 1) / L_TM, nt = (p.N + L_TN - 1) / L_TN;
-  const int pairs = (int)std::min<int64_t>(mt * nt, sms / 2);
-  const int al = out_f32 ? 4 : 8;
-  const int vec = p.ldy % al == 0 && (uintptr_t)p.y % 16 == 0;
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+// What a kernel needs once per device: its shared memory opt-in and, with
+// setmaxnreg (regs > 0), a look at the registers it is launched with:
+// setmaxnreg.inc waits for registers that a smaller launch would not have.
+template <typename K>
+int prepare_kernel(K k, int smem, int regs, int dev, std::atomic<uint64_t>& done) {
+  const uint64_t bit = dev < 64 ? UINT64_C(1) << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return DSV4_OK;
+  DSV4_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (regs) {
+    cudaFuncAttributes fa;
+    DSV4_CUDA_CHECK(cudaFuncGetAttributes(&fa, k));
+    if ((fa.numRegs + 7) / 8 * 8 < regs) return fail(DSV4_ECUDA, "fp8_matmul: built with too few registers per thread");
+  }
+  done.fetch_or(bit, std::memory_order_release);
+  return DSV4_OK;
+}
+int sm_count(int dev) {
+  static std::atomic<int> known[64];
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0 && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && dev < 64)
+    known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+template <typename K, typename... Args>
+int launch_cluster(K k, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * pairs));
-  cfg.blockDim = dim3(L_THREADS);
-  cfg.dynamicSmemBytes = L_SMEM;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster.x;
+  attr[1].val.clusterDim.y = cluster.y;
+  attr[1].val.clusterDim.z = cluster.z;
   cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  DSV4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, tx, tw, p, (int)mt, (int)nt, out_f32, vec));
+  cfg.numAttrs = cluster.x * cluster.z > 1 ? 2 : 1;
+  DSV4_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, args...));
   return DSV4_OK;
+}
+
+template <int BN, bool E8, bool A_MN>
+int launch_small(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int per, int dev, cudaStream_t st) {
+  using C = FCfg<BN, E8>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = prepare_kernel(fp8_matmul_kernel<BN, E8, A_MN>, C::SMEM, 0, dev, done)) return rc;
+  const unsigned split = (unsigned)((p.kb + per - 1) / per);
+  const dim3 grid((unsigned)((p.N + F_BM - 1) / F_BM), (unsigned)((p.M + BN - 1) / BN), split);
+  return launch_cluster(fp8_matmul_kernel<BN, E8, A_MN>, grid, C::THREADS, C::SMEM, dim3(1, 1, split), st, tw, tx, p,
+                        per);
+}
+template <int BN>
+int launch_small(bool e8, bool a_mn, const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int per, int dev,
+                 cudaStream_t st) {
+  if (e8) return a_mn ? launch_small<BN, true, true>(tw, tx, p, per, dev, st) : launch_small<BN, true, false>(tw, tx, p, per, dev, st);
+  return a_mn ? launch_small<BN, false, true>(tw, tx, p, per, dev, st) : launch_small<BN, false, false>(tw, tx, p, per, dev, st);
+}
+template <bool E8, bool B_MN>
+int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, int sms, int dev, cudaStream_t st) {
+  using C = LCfg<E8>;
+  static std::atomic<uint64_t> done{0};
+  if (int rc = prepare_kernel(fp8_matmul_pair_kernel<E8, B_MN>, C::SMEM, E8 ? 0 : C::REGS_LAUNCH, dev, done)) return rc;
+  const int64_t mt = (p.M + L_TM - 1) / L_TM, nt = (p.N + L_TN - 1) / L_TN;
+  const unsigned pairs = (unsigned)std::min<int64_t>(mt * nt, sms / 2);
+  return launch_cluster(fp8_matmul_pair_kernel<E8, B_MN>, dim3(2 * pairs), C::THREADS, C::SMEM, dim3(2, 1, 1), st, tx,
+                        tw, p, (int)mt, (int)nt);
+}
+
+// Kernel and tile of a product.
+struct Fp8Shape {
+  bool pair;
+  int bn;     // rows of a per CTA's load
+  int per;    // k-tiles per CTA of a cluster that splits K
+};
+// Few rows while the 128 x 128 tiles fit the SMs once: the cluster size then
+// fills the SMs with shares of K.  Measured (us, few rows | pairs), E8M0:
+// 300 x 1001 x 2000: 8.0 | 21.3, 512 x 4096 x 2048 (128 tiles): 10.9 | 11.3,
+// 1024 x 4096 x 4096 (256 tiles): 23.1 | 18.5, 2048^3: 14.6 | 12.7; fp32
+// scales: 8.1 | 23.8, 12.2 | 14.5, 35.9 | 24.7, 22.9 | 16.0.  Up to 128 of N a
+// pair's 256-wide tile would be half empty.
+Fp8Shape fp8_shape(int64_t m, int64_t n, int kb, int sms) {
+  Fp8Shape c = {};
+  c.bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
+  const int64_t tiles = ((n + F_BM - 1) / F_BM) * ((m + c.bn - 1) / c.bn);
+  c.pair = n > 128 && m > 128 && tiles > sms;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(8, sms / tiles));
+  // a multiple of four k-tiles each: a word of E8M0 scales
+  c.per = (int)(((kb + want - 1) / want + 3) / 4 * 4);
+  return c;
 }
 
 }  // namespace
 
 static int fp8_matmul_run(const uint8_t* a, int64_t lda, const void* as, const uint8_t* b, int64_t ldb, const void* bs,
                           int scale_type, bool trans_b, int64_t m, int64_t n, int64_t k, void* y, int64_t ldy,
-                          int out_dtype, cudaStream_t st) {
+                          int out_dtype, int dev, cudaStream_t st) {
   const int64_t kb = (k + F_BK - 1) / F_BK, nb = (n + F_BK - 1) / F_BK;
-  Fp8Params p{as, bs, trans_b ? 1 : nb, trans_b ? kb : 1, y, ldy, m, n, (int)kb,
-              scale_vec(as, (int)kb, scale_type == DSV4_SCALE_E8M0)};
-  const bool large = m > 128 && n > 128;
-  const int bn = large ? 128 : m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
+  const bool e8 = scale_type == DSV4_SCALE_E8M0, f32 = out_dtype == DSV4_DT_FP32;
+  const int sms = sm_count(dev);
+  if (sms <= 0) return fail(DSV4_ECUDA, "fp8_matmul: no SM count");
+  const Fp8Shape c = fp8_shape(m, n, (int)kb, sms);
+  // 16-byte stores of the pair kernel, four elements of the other
+  const int al = c.pair ? 16 : (f32 ? 16 : 8);
+  Fp8Params p{as, bs, trans_b ? 1 : nb, trans_b ? kb : 1, y, ldy, m, n, (int)kb, scale_vec(as, (int)kb, e8), f32,
+              (uintptr_t)y % al == 0 && ldy * (f32 ? 4 : 2) % al == 0};
   CUtensorMap tw, tx;
   const uint64_t dw[2] = {(uint64_t)(trans_b ? k : n), (uint64_t)(trans_b ? n : k)}, sw[1] = {(uint64_t)ldb};
   const uint32_t bw[2] = {128, 128};
   if (int rc = make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)b, dw, sw, bw, "fp8_matmul b")) return rc;
   const uint64_t dx[2] = {(uint64_t)k, (uint64_t)m}, sx[1] = {(uint64_t)lda};
-  const uint32_t bx[2] = {128, (uint32_t)bn};
+  const uint32_t bx[2] = {F_BK, (uint32_t)c.bn};
   if (int rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)a, dx, sx, bx, "fp8_matmul a")) return rc;
-  const bool e8 = scale_type == DSV4_SCALE_E8M0;
-  const int f32 = out_dtype == DSV4_DT_FP32;
-  if (large) {
-    int dev = 0, sms = 0;
-    DSV4_CUDA_CHECK(cudaGetDevice(&dev));
-    DSV4_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    if (e8) return trans_b ? launch_pair<true, false>(tx, tw, p, f32, sms, st) : launch_pair<true, true>(tx, tw, p, f32, sms, st);
-    return trans_b ? launch_pair<false, false>(tx, tw, p, f32, sms, st) : launch_pair<false, true>(tx, tw, p, f32, sms, st);
+  if (c.pair) {
+    if (e8) return trans_b ? launch_pair<true, false>(tx, tw, p, sms, dev, st) : launch_pair<true, true>(tx, tw, p, sms, dev, st);
+    return trans_b ? launch_pair<false, false>(tx, tw, p, sms, dev, st) : launch_pair<false, true>(tx, tw, p, sms, dev, st);
   }
-  switch (bn) {
-    case 16: return launch_small_v<16>(e8, !trans_b, tw, tx, p, f32, st);
-    case 32: return launch_small_v<32>(e8, !trans_b, tw, tx, p, f32, st);
-    case 64: return launch_small_v<64>(e8, !trans_b, tw, tx, p, f32, st);
-    default: return launch_small_v<128>(e8, !trans_b, tw, tx, p, f32, st);
+  switch (c.bn) {
+    case 16: return launch_small<16>(e8, !trans_b, tw, tx, p, c.per, dev, st);
+    case 32: return launch_small<32>(e8, !trans_b, tw, tx, p, c.per, dev, st);
+    case 64: return launch_small<64>(e8, !trans_b, tw, tx, p, c.per, dev, st);
+    default: return launch_small<128>(e8, !trans_b, tw, tx, p, c.per, dev, st);
   }
 }
 
@@ -939,7 +1179,9 @@ extern "C" int dsv4_fp8_matmul(const uint8_t* a, int64_t lda, const void* a_scal
   DSV4_CHECK_ARG(scale_type == DSV4_SCALE_E8M0 || scale_type == DSV4_SCALE_FP32, "scales must be E8M0 or fp32");
   DSV4_CHECK_ARG(out_dtype == DSV4_DT_BF16 || out_dtype == DSV4_DT_FP32, "the output is bf16 or fp32");
   DSV4_CHECK_ARG(m >= 0 && n >= 0 && k > 0, "m and n must be >= 0 and k > 0");
-  DSV4_CHECK_ARG(m <= 65535LL * 16 && n <= 0x7fffff00 && k <= 0x7fffff00, "a size is too large");
+  DSV4_CHECK_ARG(m <= 65535LL * 16 && n <= 0x7fffff00 && k <= 0x7fffff00 &&
+                     ((m + 127) / 128) * ((n + 127) / 128) <= 0x7fffffff,
+                 "a size is too large");
   DSV4_CHECK_ARG(lda >= k && ldb >= (trans_b ? k : n) && ldy >= n, "a row stride is smaller than the row");
   if (m == 0 || n == 0) return DSV4_OK;
   DSV4_CHECK_ARG(a && a_scale && b && b_scale && y, "null pointer");
@@ -951,7 +1193,54 @@ extern "C" int dsv4_fp8_matmul(const uint8_t* a, int64_t lda, const void* a_scal
   DeviceScope dev;
   if (int rc = dev.enter(a)) return rc;
   if (int rc = fp8_matmul_run(a, lda, a_scale, b, ldb, b_scale, scale_type, trans_b != 0, m, n, k, y, ldy, out_dtype,
-                              (cudaStream_t)stream))
+                              dev.device, (cudaStream_t)stream))
+    return rc;
+  DSV4_API_END
+}
+
+// Codes (rows of k bytes, padded to 16), then the scales.
+static int64_t linear_scale_offset(int64_t m, int64_t k) { return m * ((k + 15) / 16 * 16); }
+static int64_t linear_workspace(int64_t m, int64_t k, int scale_type) {
+  return linear_scale_offset(m, k) + m * ((k + 127) / 128) * (scale_type == DSV4_SCALE_E8M0 ? 1 : 4);
+}
+
+extern "C" int64_t dsv4_fp8_linear_workspace_bytes(int64_t m, int64_t k, int32_t scale_type) {
+  if (m < 0 || k <= 0 || k > 0x7fffff00 || m > 65535LL * 16 ||
+      (scale_type != DSV4_SCALE_E8M0 && scale_type != DSV4_SCALE_FP32))
+    return DSV4_EINVAL;
+  return linear_workspace(m, k, scale_type);
+}
+
+extern "C" int dsv4_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw,
+                               const void* w_scale, int32_t scale_type, int32_t trans_w, int64_t m, int64_t n,
+                               int64_t k, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+  DSV4_API_BEGIN
+  DSV4_CHECK_ARG(x_dtype == DSV4_DT_BF16 || x_dtype == DSV4_DT_FP32, "x must be bf16 or fp32");
+  DSV4_CHECK_ARG(scale_type == DSV4_SCALE_E8M0 || scale_type == DSV4_SCALE_FP32, "scales must be E8M0 or fp32");
+  DSV4_CHECK_ARG(m >= 0 && n >= 0 && k > 0, "m and n must be >= 0 and k > 0");
+  DSV4_CHECK_ARG(m <= 65535LL * 16 && n <= 0x7fffff00 && k <= 0x7fffff00 &&
+                     ((m + 127) / 128) * ((n + 127) / 128) <= 0x7fffffff,
+                 "a size is too large");
+  DSV4_CHECK_ARG(ldx >= k && ldw >= (trans_w ? k : n) && ldy >= n, "a row stride is smaller than the row");
+  if (m == 0 || n == 0) return DSV4_OK;
+  DSV4_CHECK_ARG(x && w && w_scale && y && workspace, "null pointer");
+  DSV4_CHECK_ARG((uintptr_t)w % 16 == 0 && ldw % 16 == 0, "w must start on 16 bytes, with a row stride a multiple of 16");
+  DSV4_CHECK_ARG((uintptr_t)x % (x_dtype == DSV4_DT_FP32 ? 4 : 2) == 0 &&
+                     (uintptr_t)y % (x_dtype == DSV4_DT_FP32 ? 4 : 2) == 0 &&
+                     (scale_type == DSV4_SCALE_E8M0 || (uintptr_t)w_scale % 4 == 0),
+                 "misaligned x, y or scales");
+  DSV4_CHECK_ARG((uintptr_t)workspace % 16 == 0 && workspace_bytes >= linear_workspace(m, k, scale_type),
+                 "the workspace is too small or not 16-byte aligned");
+  DeviceScope dev;
+  if (int rc = dev.enter(x)) return rc;
+  cudaStream_t st = (cudaStream_t)stream;
+  uint8_t* q = static_cast<uint8_t*>(workspace);
+  uint8_t* s = q + linear_scale_offset(m, k);
+  const int64_t ldq = (k + 15) / 16 * 16;
+  if (int rc = act_quant_fp8_launch(x, x_dtype, m, k, ldx, q, ldq, s, scale_type, st)) return rc;
+  if (int rc = fp8_matmul_run(q, ldq, s, w, ldw, w_scale, scale_type, trans_w != 0, m, n, k, y, ldy, x_dtype,
+                              dev.device, st))
     return rc;
   DSV4_API_END
 }

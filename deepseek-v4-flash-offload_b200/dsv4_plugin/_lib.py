@@ -45,6 +45,8 @@ SIGNATURES = {
     "dsv4_act_quant_mxfp4": (C.c_int, [_p, _i64, _i64, _p, _p, _p]),
     "dsv4_act_quant_fp8": (C.c_int, [_p, _i32, _i64, _i64, _i64, _p, _i64, _p, _i32, _p]),
     "dsv4_fp8_matmul": (C.c_int, [_p, _i64, _p, _p, _i64, _p, _i32, _i32, _i64, _i64, _i64, _p, _i64, _i32, _p]),
+    "dsv4_fp8_linear_workspace_bytes": (_i64, [_i64, _i64, _i32]),
+    "dsv4_fp8_linear": (C.c_int, [_p, _i32, _i64, _p, _i64, _p, _i32, _i32, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
     "dsv4_fp8_status": (C.c_int, [_i32, _p]),
     "dsv4_balance_workspace_bytes": (_i64, [_i64, _i32, _i32]),
     "dsv4_balance_forward": (C.c_int, [_p, _i32, _i64, _i32, _p, _i32, _p, _i32, _i32, _f32, _p, _p, _p, _i64, _p,

@@ -30,7 +30,13 @@ _E4M3 = torch.float8_e4m3fn
 _DT = {torch.bfloat16: DT_BF16, torch.float16: DT_FP16, torch.float32: DT_FP32}
 
 
+# the handle alone, where torch gives it: a Stream object costs 2 us a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(dev: torch.device) -> int:
+    if _raw_stream is not None and dev.index is not None:
+        return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
 
 
@@ -88,7 +94,8 @@ def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt: str | None = "u
     if scale_dtype not in (None, torch.float32) and (_E8M0 is None or scale_dtype != _E8M0 or scale_fmt is None):
         raise TypeError("scale_dtype must be float32, or float8_e8m0fnu with scale_fmt 'ue8m0'")
     _need_cuda(x)
-    x = x.detach().contiguous()
+    if not x.is_contiguous():
+        x = x.detach().contiguous()
     cols = x.shape[-1]
     rows = x.numel() // cols
     kind = SCALE_FP32 if scale_fmt is None else (SCALE_E8M0 if scale_dtype == _E8M0 else SCALE_FP32_POW2)
@@ -132,8 +139,10 @@ def _e8m0_float(s: torch.Tensor) -> torch.Tensor:
 
 def _same_device(*ts):
     _need_cuda(*ts)
-    if len({t.device for t in ts if t is not None}) > 1:
-        raise ValueError("the tensors live on different devices")
+    first = ts[0].device
+    for t in ts[1:]:
+        if t is not None and t.device != first:
+            raise ValueError("the tensors live on different devices")
 
 
 def _check_fp8_weight(b: torch.Tensor, b_scale: torch.Tensor):
@@ -199,28 +208,23 @@ def fp8_status(device=None) -> None:
 
 
 def _fp8_linear_call(x: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, trans: bool) -> torch.Tensor:
-    """act_quant(x) times w (trans: w.T) -> x's type; scales of w's type."""
+    """act_quant(x) times w (trans: w.T) -> x's type; scales of ws's type."""
     k = x.shape[-1]
-    n = w.shape[0] if trans else w.shape[1]
+    n = w.shape[0 if trans else 1]
     y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
     m = y.numel() // n if n else 0
     if m == 0:
         return y
-    x = x.detach().contiguous()
-    e8 = _is_e8m0(ws)
+    if not x.is_contiguous():
+        x = x.detach().contiguous()
     w2, ldw = _fp8_rows(w)
     sw = _fp8_scale(ws)
-    st = _stream(x.device)
-    # codes (rows padded to 16 bytes), then the scales
-    ld = (k + 15) // 16 * 16
-    nb = (k + 127) // 128
-    buf = torch.empty(m * ld + m * nb * (1 if e8 else 4), dtype=torch.uint8, device=x.device)
-    q, s = buf.data_ptr(), buf.data_ptr() + m * ld
-    kind = SCALE_E8M0 if e8 else SCALE_FP32
-    dt = _DT[x.dtype]
-    check(lib().dsv4_act_quant_fp8(x.data_ptr(), dt, m, k, k, q, ld, s, kind, st))
-    check(lib().dsv4_fp8_matmul(q, ld, s, w2.data_ptr(), ldw, sw.data_ptr(), kind, int(trans), m, n, k, y.data_ptr(), n,
-                                dt, st))
+    kind = SCALE_FP32 if sw.dtype == torch.float32 else SCALE_E8M0
+    # the codes (rows padded to 16 bytes) and the scales: dsv4_fp8_linear_workspace_bytes
+    nb = m * ((k + 15) // 16 * 16 + (k + 127) // 128 * (4 if kind == SCALE_FP32 else 1))
+    buf = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    check(lib().dsv4_fp8_linear(x.data_ptr(), _DT[x.dtype], k, w2.data_ptr(), ldw, sw.data_ptr(), kind, int(trans), m, n,
+                                k, y.data_ptr(), n, buf.data_ptr(), nb, _stream(x.device)))
     return y
 
 
@@ -231,8 +235,9 @@ class _Fp8Linear(torch.autograd.Function):
         return _fp8_linear_call(x, w, ws, True)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if dy.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("fp8_linear is differentiable once")
         w, ws = ctx.saved_tensors
         return _fp8_linear_call(dy, w, ws, False), None, None
 
@@ -352,7 +357,7 @@ class _BalanceLoss(torch.autograd.Function):
     def forward(ctx, logits, indices, offsets, n_seqs, score, alpha, status):
         t, e = logits.shape
         dev = logits.device
-        logits = logits.detach().contiguous()
+        logits = logits.contiguous()
         ws = torch.empty(int(lib().dsv4_balance_workspace_bytes(t, e, n_seqs)), dtype=torch.uint8, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         counts = torch.empty((n_seqs, e), dtype=torch.int32, device=dev)
@@ -363,15 +368,19 @@ class _BalanceLoss(torch.autograd.Function):
         ctx.save_for_backward(logits, ws)
         ctx.args = (n_seqs, score, alpha)
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)      # no zeros for the counts
         return loss, counts
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, _):
+        if grad_loss is None:
+            return None, None, None, None, None, None, None
+        if grad_loss.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("balance_loss is differentiable once")
         logits, ws = ctx.saved_tensors
         n_seqs, score, alpha = ctx.args
         t, e = logits.shape
-        up = grad_loss.float().contiguous()
+        up = grad_loss if grad_loss.dtype == torch.float32 else grad_loss.float()
         out = torch.empty_like(logits)
         check(lib().dsv4_balance_backward(logits.data_ptr(), _DT[logits.dtype], t, e, n_seqs, score, alpha,
                                           up.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
