@@ -9,12 +9,14 @@
 //   r = 1 (softmax), 1 - s (sigmoid), sigma / (2 softplus) (sqrtsoftplus).
 // The counts depend on the picks alone, so they come first and the loss is
 // then the sum of one number per token, d_t: no [sequence, expert] sums of
-// probabilities are kept.  The forward stores (row maximum, 1 / sum, d_t) per
-// token, and the backward is one pass without reductions.
+// probabilities are kept.  The forward stores (row maximum, 1 / sum, d_t,
+// sequence) per token, and the backward is one pass without reductions.
 //
 // Counts are integer atomics (any order gives the same numbers), the d_t are
-// added in double in a fixed order, so results do not depend on scheduling.
+// added in a fixed order, in double beyond a warp's rows, so results
+// do not depend on scheduling.
 // Bound: HBM, the logits once forward, once backward, the gradient once.
+// While a warp computes its rows, the next ones are on their way.
 #include <algorithm>
 
 #include "capi_internal.h"
@@ -25,22 +27,36 @@ namespace {
 
 constexpr int BL_THREADS = 256;          // 8 warps
 constexpr int BL_WARPS = BL_THREADS / 32;
-constexpr int BL_TOK = 8;                // tokens per warp: g stays in registers
-constexpr int BL_SMALL_THREADS = 512;    // the one-CTA forward
+constexpr int BL_CTAS = 4;               // per SM (64 registers a thread)
+constexpr int BL_TOK = 32;               // rows per warp at most: a lane keeps each one's state
 constexpr int BL_MAX_E = 1024;
-constexpr int64_t BL_ONE_CTA_TOKENS = 256;   // one launch up to here
+constexpr int BL_COUNT_TOK = 256;        // rows per CTA of the counts
+constexpr int BL_OFFS = 1024;            // sequence offsets kept in shared memory
+constexpr int BL_SEG = 64;               // shorter pieces of a sequence count straight in global memory
+// One CTA and one launch up to here: its counts live in shared memory.
+constexpr int BL_SMALL_THREADS = 1024;
+constexpr int BL_SMALL_TOKENS = 256;
+constexpr int BL_SMALL_COUNTS = 8192;
 
 // Saved state of one forward (the caller's buffer), then scratch.
 struct BalanceLayout {
   int64_t head;      // int[4]: sequences with tokens, CTAs done, unused, unused
   int64_t info;      // int[S][2]: tokens, picks
   int64_t hist;      // int[S][E]
-  int64_t rows;      // float4[T]: row maximum, 1 / sum (< 0: no part in the loss), d_t, sequence bits
+  int64_t rows;      // float4[T]: row maximum, 1 / sum, d_t, sequence (int bits, -1: no part in the loss)
   int64_t part;      // double[CTAs]
   int64_t bytes;
 };
-__host__ __device__ inline int64_t al16(int64_t v) { return (v + 15) / 16 * 16; }
-inline int64_t bl_ctas(int64_t T) { return (T + BL_WARPS * BL_TOK - 1) / (BL_WARPS * BL_TOK); }
+inline int64_t al16(int64_t v) { return (v + 15) / 16 * 16; }
+// Rows per warp: all CTAs on the GPU at once, up to 32 rows.
+inline int bl_tok(int64_t T) {
+  const int64_t warps = (int64_t)148 * BL_CTAS * BL_WARPS;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(BL_TOK, (T + warps - 1) / warps));
+}
+inline int64_t bl_ctas(int64_t T) {
+  const int64_t rows = (int64_t)BL_WARPS * bl_tok(T);
+  return (T + rows - 1) / rows;
+}
 inline BalanceLayout bl_layout(int64_t T, int64_t E, int64_t S) {
   BalanceLayout l;
   l.head = 0;
@@ -48,7 +64,7 @@ inline BalanceLayout bl_layout(int64_t T, int64_t E, int64_t S) {
   l.hist = l.info + al16(S * 8);
   l.rows = l.hist + al16(S * E * 4);
   l.part = l.rows + T * 16;
-  l.bytes = l.part + al16(std::max<int64_t>(bl_ctas(T), BL_SMALL_THREADS / 32) * 8);
+  l.bytes = l.part + al16(std::max<int64_t>(bl_ctas(T), 1) * 8);
   return l;
 }
 
@@ -71,16 +87,17 @@ struct BalanceParams {
   void* dlogits;
 };
 
-// The sequence of row t, -1 for a row in none (binary search).
-__device__ __forceinline__ int seq_of(const BalanceParams& p, int64_t t) {
-  if (!p.off) return 0;
-  int lo = 0, hi = p.S + 1;   // number of offsets <= t
+// The sequence of row t, -1 for a row in none (binary search); off: the
+// offsets, or their copy in shared memory.
+__device__ __forceinline__ int seq_of(const int32_t* off, int S, int64_t t) {
+  if (!off) return 0;
+  int lo = 0, hi = S + 1;   // number of offsets <= t
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if ((int64_t)p.off[mid] <= t) lo = mid + 1;
+    if ((int64_t)off[mid] <= t) lo = mid + 1;
     else hi = mid;
   }
-  return lo - 1 < p.S ? lo - 1 : -1;
+  return lo - 1 < S ? lo - 1 : -1;
 }
 
 // Offsets that descend or leave [0, T] are reported (every row still finds
@@ -93,186 +110,298 @@ __device__ void check_offsets(const BalanceParams& p) {
   }
 }
 
-// Counts of the picks of rows [t0, t1) by one CTA, one thread per token,
-// straight into the global histogram.
-__device__ void count_rows(const BalanceParams& p, int64_t t0, int64_t t1) {
-  const int lane = threadIdx.x & 31;
-  for (int64_t t = t0 + threadIdx.x; t - lane < t1; t += blockDim.x) {
-    const bool in = t < t1;
-    const int s = in ? seq_of(p, t) : -1;
-    int picks = 0;
-    for (int j = 0; j < p.k; ++j) {
-      int e = -1;
-      if (s >= 0) {
-        e = __ldcg(&p.idx[t * p.k + j]);
-        if (e < -1 || e >= p.E) {
-          set_status(p.status, DSV4_EINVAL);
-          e = -1;
-        }
-      }
-      if (e >= 0) {
-        atomicAdd(&p.hist[(int64_t)s * p.E + e], 1);
+// Adds the picks of row t of sequence s to hist[e]; returns how many count.
+__device__ __forceinline__ int count_row(const BalanceParams& p, int64_t t, int* hist) {
+  int picks = 0;
+  const int32_t* row = p.idx + t * p.k;
+  for (int j = 0; j < p.k; j += 4) {
+    int e[4] = {-1, -1, -1, -1};
+    if (p.k % 4 == 0 && (uintptr_t)p.idx % 16 == 0) {
+      const int4 v = __ldcg(reinterpret_cast<const int4*>(row + j));
+      e[0] = v.x, e[1] = v.y, e[2] = v.z, e[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i < p.k) e[i] = __ldcg(row + j + i);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (e[i] >= 0 && e[i] < p.E) {
+        atomicAdd(&hist[e[i]], 1);
         ++picks;
+      } else if (e[i] != -1) {
+        set_status(p.status, DSV4_EINVAL);
       }
     }
-    // tokens and picks per sequence: one add per group of lanes with the same sequence
-    const int key = picks ? s : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, key);
-    int sum = 0;
-    for (uint32_t r = same; r; r &= r - 1) sum += __shfl_sync(same, picks, __ffs(r) - 1);
-    if (key >= 0 && lane == __ffs(same) - 1) {
-      atomicAdd(&p.info[s].x, __popc(same));
-      atomicAdd(&p.info[s].y, sum);
-    }
+  }
+  return picks;
+}
+
+// Tokens and picks of the lanes' rows added to their sequences' totals, one
+// add per group of lanes with the same sequence.
+__device__ __forceinline__ void add_info(int2* info, int s, int picks) {
+  const int lane = threadIdx.x & 31, key = picks ? s : -1;
+  const uint32_t same = __match_any_sync(0xffffffffu, key);
+  const int sum = __reduce_add_sync(same, picks);
+  if (key >= 0 && lane == __ffs(same) - 1) {
+    atomicAdd(&info[s].x, __popc(same));
+    atomicAdd(&info[s].y, sum);
   }
 }
 
-__device__ __forceinline__ float ld_logit(const float* p) { return __ldcg(p); }
-__device__ __forceinline__ float ld_logit(const uint16_t* p) { return bf16_from_bits(__ldcg(p)); }
+__global__ void __launch_bounds__(BL_THREADS) balance_zero_kernel(int4* __restrict__ z, int64_t n16) {
+  griddep_wait();
+  griddep_launch();
+  for (int64_t i = blockIdx.x * (int64_t)BL_THREADS + threadIdx.x; i < n16; i += (int64_t)gridDim.x * BL_THREADS)
+    z[i] = make_int4(0, 0, 0, 0);
+}
 
-// Four consecutive logits of a row from column c; columns >= E give `pad`.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load4(const T* row, int c, int E, float pad, float v[4]) {
-  if constexpr (VEC) {
-    if (c < E) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 f = __ldcg(reinterpret_cast<const float4*>(row + c));
-        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+// Counts of BL_COUNT_TOK rows per CTA; every row's sequence goes to its row
+// state.  A long piece of one sequence is counted in shared memory first
+// (straight into 256 global counters, one sequence of 65536 rows took 70 us
+// more); where sequences are short, BL_SEG rows at a time go straight to
+// global memory.
+__global__ void __launch_bounds__(BL_THREADS) balance_count_kernel(const BalanceParams p) {
+  __shared__ int hist[BL_MAX_E];
+  __shared__ int32_t offs[BL_OFFS];
+  griddep_wait();
+  griddep_launch();
+  if (blockIdx.x == 0) check_offsets(p);
+  const int32_t* off = p.off;
+  if (off && p.S < BL_OFFS) {   // a search in global memory costs a microsecond
+    for (int i = threadIdx.x; i <= p.S; i += BL_THREADS) offs[i] = __ldcg(&p.off[i]);
+    __syncthreads();
+    off = offs;
+  }
+  const int64_t t0 = (int64_t)blockIdx.x * BL_COUNT_TOK, t1 = min(t0 + BL_COUNT_TOK, p.T);
+  for (int64_t a = t0; a < t1;) {   // all threads agree on the pieces
+    const int s = seq_of(off, p.S, a);
+    int64_t b = t1;
+    if (s >= 0 && off) b = max(a + 1, min((int64_t)off[s + 1], t1));
+    const bool local = s >= 0 && b - a >= BL_SEG;
+    if (local) {
+      for (int i = threadIdx.x; i < p.E; i += BL_THREADS) hist[i] = 0;
+      __syncthreads();
+    } else {
+      b = min(a + BL_SEG, t1);
+    }
+    for (int64_t t = a + threadIdx.x; t - (threadIdx.x & 31) < b; t += BL_THREADS) {
+      const int st = t >= b ? -1 : (local ? s : seq_of(off, p.S, t));
+      const int picks = st >= 0 ? count_row(p, t, local ? hist : p.hist + (int64_t)st * p.E) : 0;
+      if (t < b) p.rows[t] = make_float4(0.f, 0.f, 0.f, __int_as_float(picks ? st : -1));
+      add_info(p.info, st, picks);
+    }
+    if (local) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < p.E; i += BL_THREADS)
+        if (hist[i]) atomicAdd(&p.hist[(int64_t)s * p.E + i], hist[i]);
+      __syncthreads();
+    }
+    a = b;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// rows
+// ---------------------------------------------------------------------------
+// Lane's column j of chunk i (128 columns): four neighbours where rows take
+// vector accesses, else neighbours across the lanes.
+template <bool VEC>
+__device__ __forceinline__ int col(int i, int j) {
+  const int lane = threadIdx.x & 31;
+  return VEC ? i * 128 + lane * 4 + j : i * 128 + j * 32 + lane;
+}
+// A row's logits; columns >= E give -inf, whose score is 0.
+template <typename T, bool VEC, int NV>
+__device__ __forceinline__ void load_row(const T* row, int E, float (&v)[NV][4]) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if constexpr (VEC) {
+      const int c = col<VEC>(i, 0);
+      if (c < E) {
+        if constexpr (sizeof(T) == 4) {
+          const float4 f = __ldcg(reinterpret_cast<const float4*>(row + c));
+          v[i][0] = f.x, v[i][1] = f.y, v[i][2] = f.z, v[i][3] = f.w;
+        } else {
+          const uint2 u = __ldcg(reinterpret_cast<const uint2*>(row + c));
+          v[i][0] = bf16_from_bits(u.x & 0xffffu), v[i][1] = bf16_from_bits(u.x >> 16);
+          v[i][2] = bf16_from_bits(u.y & 0xffffu), v[i][3] = bf16_from_bits(u.y >> 16);
+        }
       } else {
-        const uint2 u = __ldcg(reinterpret_cast<const uint2*>(row + c));
-        v[0] = bf16_from_bits(u.x & 0xffffu), v[1] = bf16_from_bits(u.x >> 16);
-        v[2] = bf16_from_bits(u.y & 0xffffu), v[3] = bf16_from_bits(u.y >> 16);
+        v[i][0] = v[i][1] = v[i][2] = v[i][3] = -INFINITY;
       }
     } else {
-      v[0] = v[1] = v[2] = v[3] = pad;
-    }
-  } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = c + i < E ? ld_logit(row + c + i) : pad;
+      for (int j = 0; j < 4; ++j) {
+        const int c = col<VEC>(i, j);
+        if constexpr (sizeof(T) == 4) v[i][j] = c < E ? __ldcg(row + c) : -INFINITY;
+        else v[i][j] = c < E ? bf16_from_bits(__ldcg(row + c)) : -INFINITY;
+      }
+    }
   }
 }
 
-__device__ __forceinline__ float warp_sum_f(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// softplus(l) and e = exp(-|l|).  log1p(e) = 2 atanh(z), z = e / (2 + e) <=
+// 1/3, by its power series in z^2 <= 1/9: the first term left out is below
+// 1.5e-8 of the sum, and unlike log(1 + e) it keeps its digits as e goes to 0.
+__device__ __forceinline__ float softplus_e(float l, float* e_out) {
+  const float e = __expf(-fabsf(l));
+  const float z = __fdividef(e, 2.f + e), q = z * z;
+  float s = 1.f / 13.f;
+  s = fmaf(s, q, 1.f / 11.f);
+  s = fmaf(s, q, 1.f / 9.f);
+  s = fmaf(s, q, 1.f / 7.f);
+  s = fmaf(s, q, 1.f / 5.f);
+  s = fmaf(s, q, 1.f / 3.f);
+  s = fmaf(s, q, 1.f);
+  *e_out = e;
+  return fmaf(2.f * z, s, fmaxf(l, 0.f));
 }
-
-// Score of a logit (softmax: relative to the row maximum) and, for the
-// gradient, r with dscore/dlogit = score * r.
+// Score of a logit (softmax: relative to the row maximum mx).  The fast
+// exponential, quotient and root are each within a few 2^-23 (the exponential
+// 1.2 |l| 2^-24 more), far below the 2^-8 or so that a 1 % change of a loss
+// weight means; the library's exact ones made the kernel compute-bound.
 template <int SF>
 __device__ __forceinline__ float score_of(float l, float mx) {
-  if constexpr (SF == DSV4_SCORE_SOFTMAX) return expf(l - mx);
-  else if constexpr (SF == DSV4_SCORE_SIGMOID) return 1.f / (1.f + expf(-l));
-  else return sqrtf(fmaxf(l, 0.f) + log1pf(expf(-fabsf(l))));
-}
-template <int SF>
-__device__ __forceinline__ float score_grad(float l, float mx, float* r) {
   if constexpr (SF == DSV4_SCORE_SOFTMAX) {
-    *r = 1.f;
-    return expf(l - mx);
+    return __expf(l - mx);
   } else if constexpr (SF == DSV4_SCORE_SIGMOID) {
-    const float s = 1.f / (1.f + expf(-l));
-    *r = 1.f / (1.f + expf(l));   // 1 - s without cancellation
-    return s;
+    return __fdividef(1.f, 1.f + __expf(-l));
   } else {
-    const float e = expf(-fabsf(l));
-    const float sp = fmaxf(l, 0.f) + log1pf(e);
-    const float sg = (l >= 0.f ? 1.f : e) / (1.f + e);
-    *r = sp > 0.f ? 0.5f * sg / sp : 0.5f;   // sg / sp -> 1 far below zero
-    return sqrtf(sp);
+    float e;
+    const float sp = softplus_e(l, &e);
+    return sp > 0.f ? sp * rsqrtf(sp) : sp;   // sp: 0 or NaN
+  }
+}
+// dscore / dlogit.
+template <int SF>
+__device__ __forceinline__ float score_slope(float l, float mx) {
+  if constexpr (SF == DSV4_SCORE_SOFTMAX) {
+    return __expf(l - mx);
+  } else if constexpr (SF == DSV4_SCORE_SIGMOID) {
+    const float e = __expf(-fabsf(l)), d = 1.f + e;   // s (1 - s) = e / (1 + e)^2, either sign of l
+    return __fdividef(e, d * d);
+  } else {
+    float e;
+    const float sp = softplus_e(l, &e);
+    const float sg = __fdividef(l >= 0.f ? 1.f : e, 1.f + e);
+    return sp > 0.f ? 0.5f * sg * rsqrtf(sp) : sp;
   }
 }
 
-// Per-sequence part of g held by a warp: lane's four columns of each chunk.
-template <int NV>
+// g of one sequence, a warp's columns, from its counts.  Atomics of another
+// kernel (or of this CTA before a barrier) wrote them: global ones are read
+// past L1.
+__device__ __forceinline__ float g_factor(int2 info, int E) {
+  return info.y > 0 ? (float)E / ((float)info.x * (float)info.y) : 0.f;
+}
+template <bool VEC, int NV>
 struct GRow {
-  int seq = -2;
+  int seq = -1;
   float g[NV][4];
-  // atomics of another kernel (or of this CTA before a barrier) wrote the
-  // histogram: read it past L1
-  __device__ __forceinline__ void load(const BalanceParams& p, int s, int lane) {
-    if (s == seq) return;
+  __device__ __forceinline__ void from_counts(int s, int2 info, const int* hist, bool global, int E) {
     seq = s;
-    const int2 in = __ldcg(&p.info[s]);
-    const float c = in.y > 0 ? (float)((double)p.E / ((double)in.x * (double)in.y)) : 0.f;
+    const float c = g_factor(info, E);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = i * 128 + lane * 4 + j;
-        g[i][j] = e < p.E ? c * (float)__ldcg(&p.hist[(int64_t)s * p.E + e]) : 0.f;
+        const int e = col<VEC>(i, j);
+        g[i][j] = e < E ? c * (float)(global ? __ldcg(hist + e) : hist[e]) : 0.f;
+      }
+  }
+  __device__ __forceinline__ void from_shared(int s, const float* gs, int E) {
+    seq = s;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = col<VEC>(i, j);
+        g[i][j] = e < E ? gs[e] : 0.f;
       }
   }
 };
-
-// Whether row t has a pick (its lanes look at the k picks together).
-__device__ __forceinline__ bool row_live(const BalanceParams& p, int64_t t, int lane) {
-  bool any = false;
-  for (int j = lane; j < p.k; j += 32) {
-    const int e = __ldcg(&p.idx[t * p.k + j]);
-    any |= e >= 0 && e < p.E;
+// g of the sequence of the CTA's first row that counts, in shared memory for
+// all its warps (each warp reading it from L2 made the 1 KB of a batch's only
+// sequence the limit: 59 us instead of 31).  Returns that sequence.  `state`:
+// lanes 0 .. tok - 1 hold the sequences of the warp's rows.
+__device__ __forceinline__ int share_g(const BalanceParams& p, int mine, float* gs, int* first) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t some = __ballot_sync(0xffffffffu, mine >= 0);
+  const int s = __shfl_sync(0xffffffffu, mine, some ? __ffs(some) - 1 : 0);
+  if (lane == 0) first[warp] = some ? s : -1;
+  __syncthreads();
+  int s0 = -1;
+  for (int w = 0; w < BL_WARPS; ++w)
+    if (s0 < 0) s0 = first[w];
+  if (s0 >= 0) {
+    const float c = g_factor(__ldcg(&p.info[s0]), p.E);
+    for (int e = threadIdx.x; e < p.E; e += BL_THREADS) gs[e] = c * (float)__ldcg(&p.hist[(int64_t)s0 * p.E + e]);
   }
-  return __any_sync(0xffffffffu, any);
+  __syncthreads();
+  return s0;
 }
 
-// d_t of the rows [t0, t1) of one warp, their sum in double.
-template <typename T, bool VEC, int SF, int NV>
-__device__ double forward_rows(const BalanceParams& p, int64_t t0, int64_t t1) {
-  const int lane = threadIdx.x & 31;
-  const T* base = static_cast<const T*>(p.logits);
-  GRow<NV> gr;
-  double sum = 0.0;
-  int s = t0 < t1 ? seq_of(p, t0) : -1;
-  for (int64_t t = t0; t < t1; ++t) {
-    if (p.off) s = seq_of(p, t);
-    if (s < 0 || !row_live(p, t, lane)) {
-      if (lane == 0) p.rows[t] = make_float4(0.f, -1.f, 0.f, 0.f);
-      continue;
-    }
-    const T* row = base + t * p.E;
-    float v[NV][4];
+// d_t, row maximum and 1 / sum of R rows of the sequence in gr (together, so
+// that their reductions overlap).
+template <int SF, bool VEC, int NV, int R>
+__device__ __forceinline__ void rows_forward(float (*v)[NV][4], const GRow<VEC, NV>& gr, float (&mx)[R], float (&zi)[R],
+                                             float (&d)[R]) {
+  float z[R], u[R];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load4<T, VEC>(row, i * 128 + lane * 4, p.E, -INFINITY, v[i]);
-    gr.load(p, s, lane);
-    float mx = 0.f;
+  for (int r = 0; r < R; ++r) {
+    mx[r] = 0.f;
     if constexpr (SF == DSV4_SCORE_SOFTMAX) {
-      mx = -INFINITY;
+      mx[r] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mx = fmaxf(mx, v[i][j]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      if (mx == -INFINITY) mx = 0.f;   // every score is 0
+        for (int j = 0; j < 4; ++j) mx[r] = fmaxf(mx[r], v[r][i][j]);
     }
-    float z = 0.f, u = 0.f;
+  }
+  if constexpr (SF == DSV4_SCORE_SOFTMAX) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int r = 0; r < R; ++r) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], o));
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (mx[r] == -INFINITY) mx[r] = 0.f;   // every score is 0
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    z[r] = u[r] = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = i * 128 + lane * 4 + j;
-        const float sc = e < p.E ? score_of<SF>(v[i][j], mx) : 0.f;
-        z += sc;
-        u = fmaf(sc, gr.g[i][j], u);
+        const float sc = score_of<SF>(v[r][i][j], mx[r]);
+        z[r] += sc;
+        u[r] = fmaf(sc, gr.g[i][j], u[r]);
       }
-    z = warp_sum_f(z);
-    u = warp_sum_f(u);
-    // a row whose scores are all zero has no probabilities: no part in the loss
-    const bool none = z == 0.f;
-    const float zi = none ? -1.f : 1.f / z, d = none ? 0.f : u / z;
-    if (lane == 0) p.rows[t] = make_float4(mx, zi, d, __int_as_float(s));
-    sum += (double)d;
   }
-  return sum;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      z[r] += __shfl_xor_sync(0xffffffffu, z[r], o);
+      u[r] += __shfl_xor_sync(0xffffffffu, u[r], o);
+    }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    // a row whose scores are all zero has no probabilities: p = 0
+    zi[r] = z[r] == 0.f ? 0.f : 1.f / z[r];
+    d[r] = z[r] == 0.f ? 0.f : u[r] / z[r];
+  }
 }
 
 // Sum of the partial sums, number of sequences, loss, by one CTA.
-__device__ void finish(const BalanceParams& p, int n_part, double* red, int* redi) {
+__device__ void finish(const BalanceParams& p, const double* part, int n_part, const int2* info, double* red,
+                       int* redi) {
   double a = 0.0;
-  for (int i = threadIdx.x; i < n_part; i += blockDim.x) a += __ldcg(&p.part[i]);
+  for (int i = threadIdx.x; i < n_part; i += blockDim.x) a += __ldcg(&part[i]);
   int q = 0;
-  for (int i = threadIdx.x; i < p.S; i += blockDim.x) q += __ldcg(&p.info[i]).x > 0;
+  for (int i = threadIdx.x; i < p.S; i += blockDim.x) q += __ldcg(&info[i].x) > 0;
   red[threadIdx.x] = a;
   redi[threadIdx.x] = q;
   __syncthreads();
@@ -289,35 +418,77 @@ __device__ void finish(const BalanceParams& p, int n_part, double* red, int* red
   }
 }
 
-__global__ void __launch_bounds__(BL_THREADS) balance_zero_kernel(int4* __restrict__ z, int64_t n16) {
-  griddep_wait();
-  griddep_launch();
-  for (int64_t i = blockIdx.x * (int64_t)BL_THREADS + threadIdx.x; i < n16; i += (int64_t)gridDim.x * BL_THREADS)
-    z[i] = make_int4(0, 0, 0, 0);
-}
-
-__global__ void __launch_bounds__(BL_THREADS) balance_count_kernel(const BalanceParams p) {
-  griddep_wait();
-  griddep_launch();
-  const int64_t t0 = (int64_t)blockIdx.x * BL_THREADS;
-  if (blockIdx.x == 0) check_offsets(p);
-  count_rows(p, t0, min(t0 + BL_THREADS, p.T));
-}
-
 template <typename T, bool VEC, int SF, int NV>
-__global__ void __launch_bounds__(BL_THREADS) balance_forward_kernel(const BalanceParams p) {
+__global__ void __launch_bounds__(BL_THREADS, NV <= 2 ? BL_CTAS : 1) balance_forward_kernel(const BalanceParams p, const int tok) {
   __shared__ double red[BL_THREADS];
   __shared__ int redi[BL_THREADS];
+  __shared__ float gs[BL_MAX_E];
   __shared__ int last;
+  constexpr int BATCH = NV == 1 ? 4 : (NV == 2 ? 2 : 1);   // rows computed together
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t0 = ((int64_t)blockIdx.x * BL_WARPS + warp) * tok;
+  const int n = (int)max((int64_t)0, min((int64_t)tok, p.T - t0));
+  const T* rows = static_cast<const T*>(p.logits) + t0 * p.E;
+  float v[BATCH][NV][4], nx[BATCH][NV][4];
+  // Before the wait: the kernel just before is this call's count kernel, which
+  // does not write logits, and it starts its successor only after its own wait,
+  // when whatever wrote them is complete.
+#pragma unroll
+  for (int r = 0; r < BATCH; ++r)
+    if (r < n) load_row<T, VEC, NV>(rows + (int64_t)r * p.E, p.E, nx[r]);
   griddep_wait();
   griddep_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t0 = ((int64_t)blockIdx.x * BL_WARPS + warp) * BL_TOK;
-  const double d = forward_rows<T, VEC, SF, NV>(p, min(t0, p.T), min(t0 + BL_TOK, p.T));
+  const int mine = lane < n ? __float_as_int(__ldcg(&p.rows[t0 + lane].w)) : -1;
+  const int s0 = share_g(p, mine, gs, redi);
+  GRow<VEC, NV> gr;
+  float sum = 0.f;
+  float4 state = make_float4(0.f, 0.f, 0.f, __int_as_float(mine));   // lane i: row t0 + i
+#pragma unroll 1
+  for (int b = 0; b < n; b += BATCH) {
+#pragma unroll
+    for (int r = 0; r < BATCH; ++r) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[r][i][j] = nx[r][i][j];
+      if (b + BATCH + r < n) load_row<T, VEC, NV>(rows + (int64_t)(b + BATCH + r) * p.E, p.E, nx[r]);
+    }
+    int s[BATCH];
+    bool other = false;
+#pragma unroll
+    for (int r = 0; r < BATCH; ++r) {
+      s[r] = b + r < n ? __shfl_sync(0xffffffffu, mine, (b + r) & 31) : -1;
+      other |= s[r] >= 0 && s[r] != gr.seq;
+    }
+    float mx[BATCH], zi[BATCH], d[BATCH];
+    if (!other) {
+      rows_forward<SF, VEC, NV, BATCH>(v, gr, mx, zi, d);
+    } else {
+#pragma unroll
+      for (int r = 0; r < BATCH; ++r) {
+        if (s[r] < 0) continue;
+        if (s[r] != gr.seq) {
+          if (s[r] == s0) gr.from_shared(s[r], gs, p.E);
+          else gr.from_counts(s[r], __ldcg(&p.info[s[r]]), p.hist + (int64_t)s[r] * p.E, true, p.E);
+        }
+        float m1[1], z1[1], d1[1];
+        rows_forward<SF, VEC, NV, 1>(v + r, gr, m1, z1, d1);
+        mx[r] = m1[0], zi[r] = z1[0], d[r] = d1[0];
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < BATCH; ++r) {
+      if (s[r] < 0) continue;
+      if (lane == b + r) state = make_float4(mx[r], zi[r], d[r], __int_as_float(s[r]));
+      sum += d[r];
+    }
+  }
+  if (lane < n) p.rows[t0 + lane] = state;
   for (int64_t i = blockIdx.x * (int64_t)BL_THREADS + threadIdx.x; i < (int64_t)p.S * p.E;
        i += (int64_t)gridDim.x * BL_THREADS)
     p.counts[i] = __ldcg(&p.hist[i]);
-  if (lane == 0) red[warp] = d;
+  __syncthreads();
+  if (lane == 0) red[warp] = (double)sum;
   __syncthreads();
   if (threadIdx.x == 0) {
     double a = 0.0;
@@ -329,102 +500,175 @@ __global__ void __launch_bounds__(BL_THREADS) balance_forward_kernel(const Balan
   __syncthreads();
   if (!last) return;
   __threadfence();
-  finish(p, gridDim.x, red, redi);
+  finish(p, p.part, gridDim.x, p.info, red, redi);
 }
 
 // Small batches: counts, loss and row statistics in one CTA and one launch.
 template <typename T, bool VEC, int SF, int NV>
 __global__ void __launch_bounds__(BL_SMALL_THREADS) balance_forward_small_kernel(const BalanceParams p) {
+  extern __shared__ int hist[];            // [S][E] counts, then [S] (tokens, picks)
+  __shared__ int row_seq[BL_SMALL_TOKENS];
   __shared__ double red[BL_SMALL_THREADS];
   __shared__ int redi[BL_SMALL_THREADS];
   griddep_wait();
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  for (int64_t i = threadIdx.x; i < (int64_t)p.S * p.E; i += blockDim.x) p.hist[i] = 0;
-  for (int i = threadIdx.x; i < p.S; i += blockDim.x) p.info[i] = make_int2(0, 0);
-  __threadfence();
+  const int n = p.S * p.E, T_ = (int)p.T;
+  int2* info = reinterpret_cast<int2*>(hist + (n + 1) / 2 * 2);
+  // the first row of this warp is on its way while the picks are counted
+  float v[NV][4];
+  if (warp < T_) load_row<T, VEC, NV>(static_cast<const T*>(p.logits) + (int64_t)warp * p.E, p.E, v);
+  for (int i = threadIdx.x; i < n; i += blockDim.x) hist[i] = 0;
+  for (int i = threadIdx.x; i < p.S; i += blockDim.x) info[i] = make_int2(0, 0);
   __syncthreads();
   check_offsets(p);
-  count_rows(p, 0, p.T);
-  __threadfence();
+  if (threadIdx.x < BL_SMALL_TOKENS) {
+    const int t = threadIdx.x, s = t < T_ ? seq_of(p.off, p.S, t) : -1;
+    const int picks = s >= 0 ? count_row(p, t, hist + s * p.E) : 0;
+    row_seq[t] = picks ? s : -1;
+    add_info(info, s, picks);
+  }
   __syncthreads();
-  for (int64_t i = threadIdx.x; i < (int64_t)p.S * p.E; i += blockDim.x) p.counts[i] = __ldcg(&p.hist[i]);
-  const int64_t per = (p.T + nw - 1) / nw, t0 = warp * per;
-  const double d = forward_rows<T, VEC, SF, NV>(p, min(t0, p.T), min(t0 + per, p.T));
-  if (lane == 0) p.part[warp] = d;
-  __threadfence();
+  for (int i = threadIdx.x; i < n; i += blockDim.x) p.counts[i] = p.hist[i] = hist[i];
+  for (int i = threadIdx.x; i < p.S; i += blockDim.x) p.info[i] = info[i];
+  GRow<VEC, NV> gr;
+  float sum = 0.f;
+  for (int t = warp; t < T_; t += nw) {
+    if (t != warp) load_row<T, VEC, NV>(static_cast<const T*>(p.logits) + (int64_t)t * p.E, p.E, v);
+    const int s = row_seq[t];
+    float mx = 0.f, zi = 0.f, d = 0.f;
+    if (s >= 0) {
+      if (s != gr.seq) gr.from_counts(s, info[s], hist + s * p.E, false, p.E);
+      float m1[1], z1[1], d1[1];
+      rows_forward<SF, VEC, NV, 1>(&v, gr, m1, z1, d1);
+      mx = m1[0], zi = z1[0], d = d1[0];
+    }
+    if (lane == 0) p.rows[t] = make_float4(mx, zi, d, __int_as_float(s));
+    sum += d;
+  }
   __syncthreads();
-  finish(p, nw, red, redi);
+  red[threadIdx.x] = lane == 0 ? (double)sum : 0.0;
+  int q = 0;
+  for (int i = threadIdx.x; i < p.S; i += blockDim.x) q += info[i].x > 0;
+  redi[threadIdx.x] = q;
+  __syncthreads();
+  if (warp == 0) {
+    double a = red[lane * 32];             // warp w's sum is at 32 w
+    q = 0;
+    for (int i = lane; i < (int)blockDim.x; i += 32) q += redi[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(0xffffffffu, a, o);
+      q += __shfl_xor_sync(0xffffffffu, q, o);
+    }
+    if (lane == 0) {
+      p.head[0] = q;
+      *p.loss = q ? (float)((double)p.alpha * a / q) : 0.f;
+    }
+  }
 }
 
 template <typename T, bool VEC, int SF, int NV>
-__global__ void __launch_bounds__(BL_THREADS) balance_backward_kernel(const BalanceParams p) {
+__global__ void __launch_bounds__(BL_THREADS, NV <= 2 ? BL_CTAS : 1) balance_backward_kernel(const BalanceParams p, const int tok) {
+  __shared__ float gs[BL_MAX_E];
+  __shared__ int first[BL_WARPS];
+  constexpr int BATCH = NV == 1 ? 4 : (NV == 2 ? 2 : 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t0 = ((int64_t)blockIdx.x * BL_WARPS + warp) * tok;
+  const int n = (int)max((int64_t)0, min((int64_t)tok, p.T - t0));
+  const T* rows = static_cast<const T*>(p.logits) + t0 * p.E;
   griddep_wait();
   griddep_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t0 = ((int64_t)blockIdx.x * BL_WARPS + warp) * BL_TOK, t1 = min(t0 + BL_TOK, p.T);
+  float v[BATCH][NV][4], nx[BATCH][NV][4];
+#pragma unroll
+  for (int r = 0; r < BATCH; ++r)
+    if (r < n) load_row<T, VEC, NV>(rows + (int64_t)r * p.E, p.E, nx[r]);
+  const float4 state = lane < n ? __ldcg(&p.rows[t0 + lane]) : make_float4(0.f, 0.f, 0.f, __int_as_float(-1));
   const int q = __ldcg(&p.head[0]);
   const float c = q ? p.alpha / (float)q * __ldcg(p.up) : 0.f;
-  GRow<NV> gr;
-  for (int64_t t = t0; t < t1; ++t) {
-    const float4 st = __ldcg(&p.rows[t]);
-    const bool live = st.y >= 0.f || st.y != st.y;
-    float o[NV][4];
-    if (live) {
-      const T* row = static_cast<const T*>(p.logits) + t * p.E;
-      float v[NV][4];
+  const int s0 = share_g(p, __float_as_int(state.w), gs, first);
+  GRow<VEC, NV> gr;
+#pragma unroll 1
+  for (int b = 0; b < n; b += BATCH) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) load4<T, VEC>(row, i * 128 + lane * 4, p.E, 0.f, v[i]);
-      gr.load(p, __float_as_int(st.w), lane);
+    for (int r = 0; r < BATCH; ++r) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          float r;
-          const float s = score_grad<SF>(v[i][j], st.x, &r);
-          o[i][j] = c * (s * st.y) * r * (gr.g[i][j] - st.z);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int j = 0; j < 4; ++j) v[r][i][j] = nx[r][i][j];
+      if (b + BATCH + r < n) load_row<T, VEC, NV>(rows + (int64_t)(b + BATCH + r) * p.E, p.E, nx[r]);
     }
-    T* dst = static_cast<T*>(p.dlogits) + t * p.E;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int e = i * 128 + lane * 4;
-      if constexpr (VEC) {
-        if (e < p.E) {
-          if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4*>(dst + e) = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
-          else
-            *reinterpret_cast<uint2*>(dst + e) = make_uint2(bf16_bits(o[i][0]) | ((uint32_t)bf16_bits(o[i][1]) << 16),
-                                                            bf16_bits(o[i][2]) | ((uint32_t)bf16_bits(o[i][3]) << 16));
+    for (int r = 0; r < BATCH; ++r) {
+      if (b + r >= n) break;
+      const float mx = __shfl_sync(0xffffffffu, state.x, (b + r) & 31);
+      const float zc = c * __shfl_sync(0xffffffffu, state.y, (b + r) & 31);
+      const float d = __shfl_sync(0xffffffffu, state.z, (b + r) & 31);
+      const int s = __float_as_int(__shfl_sync(0xffffffffu, state.w, (b + r) & 31));
+      if (s >= 0) {
+        if (s != gr.seq) {
+          if (s == s0) gr.from_shared(s, gs, p.E);
+          else gr.from_counts(s, __ldcg(&p.info[s]), p.hist + (int64_t)s * p.E, true, p.E);
         }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[r][i][j] = zc * score_slope<SF>(v[r][i][j], mx) * (gr.g[i][j] - d);
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (e + j < p.E) {
-            if constexpr (sizeof(T) == 4) dst[e + j] = o[i][j];
-            else dst[e + j] = bf16_bits(o[i][j]);
+        for (int i = 0; i < NV; ++i) v[r][i][0] = v[r][i][1] = v[r][i][2] = v[r][i][3] = 0.f;
+      }
+      T* dst = static_cast<T*>(p.dlogits) + (t0 + b + r) * p.E;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float* o = v[r][i];
+        if constexpr (VEC) {
+          const int e = col<VEC>(i, 0);
+          if (e < p.E) {
+            if constexpr (sizeof(T) == 4)
+              *reinterpret_cast<float4*>(dst + e) = make_float4(o[0], o[1], o[2], o[3]);
+            else
+              *reinterpret_cast<uint2*>(dst + e) =
+                  make_uint2(bf16_bits(o[0]) | ((uint32_t)bf16_bits(o[1]) << 16),
+                             bf16_bits(o[2]) | ((uint32_t)bf16_bits(o[3]) << 16));
           }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int e = col<VEC>(i, j);
+            if (e < p.E) {
+              if constexpr (sizeof(T) == 4) dst[e] = o[j];
+              else dst[e] = bf16_bits(o[j]);
+            }
+          }
+        }
       }
     }
   }
 }
 
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
 enum Pass { FORWARD, FORWARD_SMALL, BACKWARD };
 
 template <typename T, bool VEC, int SF, int NV>
 cudaError_t launch_pass(Pass pass, const BalanceParams& p, cudaStream_t st) {
   const dim3 grid((unsigned)std::max<int64_t>(bl_ctas(p.T), 1));
   if (pass == FORWARD)
-    return launch_k(balance_forward_kernel<T, VEC, SF, NV>, grid, dim3(BL_THREADS), 0, st, pdl_enabled(), p);
-  if (pass == FORWARD_SMALL)
-    return launch_k(balance_forward_small_kernel<T, VEC, SF, NV>, dim3(1), dim3(BL_SMALL_THREADS), 0, st, pdl_enabled(), p);
-  return launch_k(balance_backward_kernel<T, VEC, SF, NV>, grid, dim3(BL_THREADS), 0, st, pdl_enabled(), p);
+    return launch_k(balance_forward_kernel<T, VEC, SF, NV>, grid, dim3(BL_THREADS), 0, st, pdl_enabled(), p,
+                    bl_tok(p.T));
+  if (pass == FORWARD_SMALL) {
+    const size_t smem = ((size_t)p.S * p.E + 1) / 2 * 8 + (size_t)p.S * 8;
+    return launch_k(balance_forward_small_kernel<T, VEC, SF, NV>, dim3(1), dim3(BL_SMALL_THREADS), smem, st,
+                    pdl_enabled(), p);
+  }
+  return launch_k(balance_backward_kernel<T, VEC, SF, NV>, grid, dim3(BL_THREADS), 0, st, pdl_enabled(), p,
+                  bl_tok(p.T));
 }
 template <typename T, bool VEC, int SF>
 cudaError_t launch_nv(Pass pass, const BalanceParams& p, cudaStream_t st) {
+  if (p.E <= 128) return launch_pass<T, VEC, SF, 1>(pass, p, st);
   if (p.E <= 256) return launch_pass<T, VEC, SF, 2>(pass, p, st);
   if (p.E <= 512) return launch_pass<T, VEC, SF, 4>(pass, p, st);
   return launch_pass<T, VEC, SF, 8>(pass, p, st);
@@ -493,7 +737,7 @@ extern "C" int dsv4_balance_forward(const void* logits, int32_t dtype, int64_t n
   BalanceParams p = bl_params(workspace, n_tokens, n_experts, n_seqs);
   p.logits = logits, p.idx = indices, p.k = topk, p.off = seq_offsets, p.score = score_func, p.alpha = alpha;
   p.loss = loss, p.counts = counts, p.status = status;
-  if (n_tokens <= BL_ONE_CTA_TOKENS && (int64_t)n_seqs * n_experts <= 16384) {
+  if (n_tokens <= BL_SMALL_TOKENS && (int64_t)n_seqs * (n_experts + 2) <= BL_SMALL_COUNTS) {
     DSV4_CUDA_CHECK(launch(FORWARD_SMALL, dtype, p, st));
     return DSV4_OK;
   }
@@ -502,7 +746,7 @@ extern "C" int dsv4_balance_forward(const void* logits, int32_t dtype, int64_t n
   DSV4_CUDA_CHECK(launch_k(balance_zero_kernel, dim3(zc), dim3(BL_THREADS), 0, st, pdl_enabled(),
                            static_cast<int4*>(workspace), n16));
   if (n_tokens > 0)
-    DSV4_CUDA_CHECK(launch_k(balance_count_kernel, dim3((unsigned)((n_tokens + BL_THREADS - 1) / BL_THREADS)),
+    DSV4_CUDA_CHECK(launch_k(balance_count_kernel, dim3((unsigned)((n_tokens + BL_COUNT_TOK - 1) / BL_COUNT_TOK)),
                              dim3(BL_THREADS), 0, st, pdl_enabled(), p));
   DSV4_CUDA_CHECK(launch(FORWARD, dtype, p, st));
   DSV4_API_END
