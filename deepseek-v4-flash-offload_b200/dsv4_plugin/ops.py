@@ -99,9 +99,8 @@ def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt: str | None = "u
     cols = x.shape[-1]
     rows = x.numel() // cols
     kind = SCALE_FP32 if scale_fmt is None else (SCALE_E8M0 if scale_dtype == _E8M0 else SCALE_FP32_POW2)
-    q = torch.empty(x.shape, dtype=_E4M3, device=x.device)
-    s = torch.empty((*x.shape[:-1], (cols + 127) // 128), dtype=_E8M0 if kind == SCALE_E8M0 else torch.float32,
-                    device=x.device)
+    q = x.new_empty(x.shape, dtype=_E4M3)
+    s = x.new_empty((*x.shape[:-1], (cols + 127) // 128), dtype=_E8M0 if kind == SCALE_E8M0 else torch.float32)
     check(lib().dsv4_act_quant_fp8(x.data_ptr(), _DT[x.dtype], rows, cols, cols, q.data_ptr(), cols, s.data_ptr(), kind,
                                    _stream(x.device)))
     return q, s
@@ -182,8 +181,7 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
         a_scale, b_scale = (_e8m0_float(a_scale), b_scale) if e8 else (a_scale, _e8m0_float(b_scale))
         e8 = False
     _same_device(a, a_scale, b, b_scale)
-    dev = a.device
-    y = torch.empty((*a.shape[:-1], n), dtype=out_dtype, device=dev)
+    y = a.new_empty((*a.shape[:-1], n), dtype=out_dtype)
     m = y.numel() // n if n else 0
     if m == 0:
         return y
@@ -192,7 +190,7 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     sa, sb = _fp8_scale(a_scale), _fp8_scale(b_scale)
     check(lib().dsv4_fp8_matmul(a2.data_ptr(), lda, sa.data_ptr(), b2.data_ptr(), ldb, sb.data_ptr(),
                                 SCALE_E8M0 if e8 else SCALE_FP32, int(bool(trans_b)), m, n, k, y.data_ptr(), n,
-                                _DT[out_dtype], _stream(dev)))
+                                _DT[out_dtype], _stream(a.device)))
     return y
 
 
@@ -211,7 +209,7 @@ def _fp8_linear_call(x: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, trans: 
     """act_quant(x) times w (trans: w.T) -> x's type; scales of ws's type."""
     k = x.shape[-1]
     n = w.shape[0 if trans else 1]
-    y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], n))
     m = y.numel() // n if n else 0
     if m == 0:
         return y
@@ -222,7 +220,7 @@ def _fp8_linear_call(x: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, trans: 
     kind = SCALE_FP32 if sw.dtype == torch.float32 else SCALE_E8M0
     # the codes (rows padded to 16 bytes) and the scales: dsv4_fp8_linear_workspace_bytes
     nb = m * ((k + 15) // 16 * 16 + (k + 127) // 128 * (4 if kind == SCALE_FP32 else 1))
-    buf = torch.empty(nb, dtype=torch.uint8, device=x.device)
+    buf = x.new_empty((nb + 1) // 2)       # x's type: at least two bytes an element
     check(lib().dsv4_fp8_linear(x.data_ptr(), _DT[x.dtype], k, w2.data_ptr(), ldw, sw.data_ptr(), kind, int(trans), m, n,
                                 k, y.data_ptr(), n, buf.data_ptr(), nb, _stream(x.device)))
     return y
@@ -356,15 +354,15 @@ class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, indices, offsets, n_seqs, score, alpha, status):
         t, e = logits.shape
-        dev = logits.device
         logits = logits.contiguous()
-        ws = torch.empty(int(lib().dsv4_balance_workspace_bytes(t, e, n_seqs)), dtype=torch.uint8, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        counts = torch.empty((n_seqs, e), dtype=torch.int32, device=dev)
+        nb = lib().dsv4_balance_workspace_bytes(t, e, n_seqs)
+        ws = logits.new_empty(nb, dtype=torch.uint8)
+        loss = logits.new_empty((), dtype=torch.float32)
+        counts = logits.new_empty(e if offsets is None else (n_seqs, e), dtype=torch.int32)
         check(lib().dsv4_balance_forward(logits.data_ptr(), _DT[logits.dtype], t, e, indices.data_ptr(),
                                          indices.shape[1], None if offsets is None else offsets.data_ptr(), n_seqs,
-                                         score, alpha, loss.data_ptr(), counts.data_ptr(), ws.data_ptr(), ws.numel(),
-                                         None if status is None else status.data_ptr(), _stream(dev)))
+                                         score, alpha, loss.data_ptr(), counts.data_ptr(), ws.data_ptr(), nb,
+                                         None if status is None else status.data_ptr(), _stream(logits.device)))
         ctx.save_for_backward(logits, ws)
         ctx.args = (n_seqs, score, alpha)
         ctx.mark_non_differentiable(counts)
@@ -432,7 +430,7 @@ def balance_loss(logits: torch.Tensor, indices: torch.Tensor, score_func: str = 
         seq_offsets = seq_offsets.contiguous()
     loss, counts = _BalanceLoss.apply(logits, indices.contiguous(), seq_offsets, n_seqs, SCORE_FUNCS[score_func],
                                       float(alpha), status)
-    return loss, counts if seq_offsets is not None else counts[0]
+    return loss, counts
 
 
 def combine_ordered(rows: torch.Tensor, order: torch.Tensor) -> torch.Tensor:
