@@ -35,6 +35,7 @@ constexpr int F_BM = 128;              // of N (weight rows) per CTA
 constexpr int F_GROUP = 4;             // k-tiles per scale group
 constexpr int F_SLOTS = 4;             // scale groups in flight
 constexpr int F_EPI_WARP0 = 4;
+constexpr int64_t F_MAX_M = 65535LL * 128;   // grid y, in tiles of 128 rows
 
 // Set by a kernel whose bounded wait ran out; read by dsv4_fp8_status.
 __device__ int g_fp8_status;
@@ -1201,7 +1202,7 @@ extern "C" int dsv4_fp8_matmul(const uint8_t* a, int64_t lda, const void* a_scal
   DSV4_CHECK_ARG(scale_type == DSV4_SCALE_E8M0 || scale_type == DSV4_SCALE_FP32, "scales must be E8M0 or fp32");
   DSV4_CHECK_ARG(out_dtype == DSV4_DT_BF16 || out_dtype == DSV4_DT_FP32, "the output is bf16 or fp32");
   DSV4_CHECK_ARG(m >= 0 && n >= 0 && k > 0, "m and n must be >= 0 and k > 0");
-  DSV4_CHECK_ARG(m <= 65535LL * 16 && n <= 0x7fffff00 && k <= 0x7fffff00 &&
+  DSV4_CHECK_ARG(m <= F_MAX_M && n <= 0x7fffff00 && k <= 0x7fffff00 &&
                      ((m + 127) / 128) * ((n + 127) / 128) <= 0x7fffffff,
                  "a size is too large");
   DSV4_CHECK_ARG(lda >= k && ldb >= (trans_b ? k : n) && ldy >= n, "a row stride is smaller than the row");
@@ -1227,7 +1228,7 @@ static int64_t linear_workspace(int64_t m, int64_t k, int scale_type) {
 }
 
 extern "C" int64_t dsv4_fp8_linear_workspace_bytes(int64_t m, int64_t k, int32_t scale_type) {
-  if (m < 0 || k <= 0 || k > 0x7fffff00 || m > 65535LL * 16 ||
+  if (m < 0 || k <= 0 || k > 0x7fffff00 || m > F_MAX_M ||
       (scale_type != DSV4_SCALE_E8M0 && scale_type != DSV4_SCALE_FP32))
     return DSV4_EINVAL;
   return linear_workspace(m, k, scale_type);
@@ -1241,7 +1242,7 @@ extern "C" int dsv4_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, cons
   DSV4_CHECK_ARG(x_dtype == DSV4_DT_BF16 || x_dtype == DSV4_DT_FP32, "x must be bf16 or fp32");
   DSV4_CHECK_ARG(scale_type == DSV4_SCALE_E8M0 || scale_type == DSV4_SCALE_FP32, "scales must be E8M0 or fp32");
   DSV4_CHECK_ARG(m >= 0 && n >= 0 && k > 0, "m and n must be >= 0 and k > 0");
-  DSV4_CHECK_ARG(m <= 65535LL * 16 && n <= 0x7fffff00 && k <= 0x7fffff00 &&
+  DSV4_CHECK_ARG(m <= F_MAX_M && n <= 0x7fffff00 && k <= 0x7fffff00 &&
                      ((m + 127) / 128) * ((n + 127) / 128) <= 0x7fffffff,
                  "a size is too large");
   DSV4_CHECK_ARG(ldx >= k && ldw >= (trans_w ? k : n) && ldy >= n, "a row stride is smaller than the row");

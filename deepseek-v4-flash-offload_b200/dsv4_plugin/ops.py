@@ -110,6 +110,8 @@ def _fp8_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """(FP8 matrix the kernels can read, its row stride in bytes): rows that
     start on 16 bytes, columns next to each other; copied when it is not."""
     r, c = t.shape
+    if c % 16 == 0 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, c
     ld = t.stride(0) if r > 1 else (c + 15) // 16 * 16
     if (t.stride(1) == 1 or c == 1) and ld % 16 == 0 and ld >= c and t.data_ptr() % 16 == 0:
         return t, ld
@@ -125,11 +127,12 @@ def _fp8_scale(s: torch.Tensor) -> torch.Tensor:
 
 
 def _is_e8m0(s: torch.Tensor) -> bool:
-    if s.dtype == torch.float32:
+    dt = s.dtype
+    if dt == torch.float32:
         return False
-    if s.dtype == torch.uint8 or (_E8M0 is not None and s.dtype == _E8M0):
+    if dt == torch.uint8 or (_E8M0 is not None and dt == _E8M0):
         return True
-    raise TypeError(f"FP8 scales are float32 or E8M0 (float8_e8m0fnu or uint8), got {s.dtype}")
+    raise TypeError(f"FP8 scales are float32 or E8M0 (float8_e8m0fnu or uint8), got {dt}")
 
 
 def _e8m0_float(s: torch.Tensor) -> torch.Tensor:
@@ -147,7 +150,7 @@ def _same_device(*ts):
 def _check_fp8_weight(b: torch.Tensor, b_scale: torch.Tensor):
     if b.dtype != _E4M3:
         raise TypeError(f"expected a float8_e4m3fn matrix, got {b.dtype}")
-    if b.dim() != 2 or tuple(b_scale.shape) != ((b.shape[0] + 127) // 128, (b.shape[1] + 127) // 128):
+    if b.dim() != 2 or b_scale.shape != ((b.shape[0] + 127) // 128, (b.shape[1] + 127) // 128):
         raise ValueError(f"a matrix of shape {tuple(b.shape)} needs one scale per 128 x 128 block, "
                          f"got {tuple(b_scale.shape)}")
 
@@ -171,10 +174,10 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale:
     if a.dim() < 1 or a.shape[-1] == 0:
         raise ValueError("fp8_matmul needs K > 0")
     k = a.shape[-1]
-    n, kb = (b.shape[0], b.shape[1]) if trans_b else (b.shape[1], b.shape[0])
+    n, kb = b.shape if trans_b else b.shape[::-1]
     if kb != k:
         raise ValueError(f"a has K = {k}, b has K = {kb}")
-    if tuple(a_scale.shape) != (*a.shape[:-1], (k + 127) // 128):
+    if a_scale.shape != (*a.shape[:-1], (k + 127) // 128):
         raise ValueError(f"a_scale must be {(*a.shape[:-1], (k + 127) // 128)}, got {tuple(a_scale.shape)}")
     e8 = _is_e8m0(a_scale)
     if e8 != _is_e8m0(b_scale):

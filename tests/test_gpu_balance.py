@@ -108,6 +108,58 @@ def test_packed_sequences(ops, fn, t, off):
     assert (grad[(idx < 0).all(1)] == 0).all()
 
 
+@pytest.mark.parametrize("t,s", [(20000, 20000), (5000, 1500), (70000, 3)])
+def test_many_sequences(ops, t, s):
+    """A sequence per token; sequences around the piece that is counted in
+    shared memory; more rows per warp than a batch."""
+    g = np.random.RandomState(t)
+    cuts = np.sort(g.randint(0, t + 1, s - 1)).tolist() if s != t else list(range(1, t))
+    lg, idx = make(t, t, 16, 2, spread=1.0)
+    off = [0, *cuts, t]
+    offs = torch.tensor(off, device="cuda")
+    x = lg.clone().requires_grad_(True)
+    loss, counts = ops.balance_loss(x, idx, "sigmoid", 1.0, offs)
+    grad, = torch.autograd.grad(loss, x)
+    # the definition over all rows at once (a loop over sequences would be slow)
+    l64 = lg.double().requires_grad_(True)
+    p = torch.sigmoid(l64)
+    p = p / p.sum(1, keepdim=True)
+    seq = torch.bucketize(torch.arange(t, device="cuda"), offs, right=True) - 1
+    live = (idx >= 0).any(1)
+    c = torch.zeros(s * 16, dtype=torch.int64, device="cuda")
+    c = c.index_add_(0, (seq[:, None] * 16 + idx)[live].reshape(-1), torch.ones(int(live.sum()) * 2, dtype=torch.int64,
+                                                                               device="cuda")).view(s, 16)
+    n = torch.zeros(s, dtype=torch.int64, device="cuda").index_add_(0, seq[live], torch.ones_like(seq[live]))
+    f = c.double() * 16 / c.sum(1, keepdim=True).clamp(min=1) / n.clamp(min=1)[:, None]
+    want = (f[seq] * p)[live].sum() / (n > 0).sum()
+    gw, = torch.autograd.grad(want, l64)
+    assert torch.equal(counts.long(), c)
+    U = (96 + 2 * float(lg.abs().max())) * 2.0 ** -24
+    assert abs(float(loss.detach()) - float(want.detach())) <= (U + 2.0 ** -24) * float(want.detach())
+    gg = f[seq] / (n > 0).sum()
+    tol = U * p.detach() * (gg + (gg * p.detach()).sum(1, keepdim=True))
+    assert ((grad.double() - gw).abs() <= tol + 1e-45).all()
+
+
+def test_offsets_beyond_32_bits(ops):
+    """Logits of more than 2^32 bytes: the last sequence as computed alone."""
+    t, e, tail = 8_500_000, 256, 1000
+    lg = torch.zeros((t, e), dtype=torch.bfloat16, device="cuda")
+    last, idx_last = make(1, tail, e, 8, torch.bfloat16, pad=0.0)
+    lg[-tail:] = last
+    idx = torch.full((t, 8), -1, dtype=torch.int32, device="cuda")
+    idx[-tail:] = idx_last
+    x = lg.requires_grad_(True)
+    loss, counts = ops.balance_loss(x, idx, "sigmoid")
+    grad, = torch.autograd.grad(loss, x)
+    y = last.clone().requires_grad_(True)
+    l2, c2 = ops.balance_loss(y, idx_last, "sigmoid")
+    g2, = torch.autograd.grad(l2, y)
+    assert torch.equal(counts, c2) and abs(float(loss.detach()) - float(l2.detach())) <= 2.0 ** -20 * float(l2.detach())
+    assert torch.equal(grad[-tail:], g2)
+    assert not grad[:-tail].any()
+
+
 @pytest.mark.parametrize("t", [40, 900])
 def test_nothing_counts(ops, t):
     """Only padding; and no rows at all."""

@@ -219,6 +219,103 @@ def test_fp8_matmul_unaligned_is_copied(ops, e8):
         check_product(y5, deq64(q, s, False), deq64(wt, bs[:, :2].t(), True), 256)
 
 
+@pytest.mark.parametrize("e8", [True, False])
+@pytest.mark.parametrize("k", [128, 1024, 1536, 2048, 2560, 3000, 3584, 4096, 4104, 12288])
+def test_fp8_matmul_every_cluster_size(ops, k, e8):
+    """K split over 1 to 8 CTAs, with shares that end inside a group of scales."""
+    for m in (1, 40, 128):
+        q, s = ops.act_quant(activations(k + m, m, k), 128, "ue8m0" if e8 else None, E8 if e8 else None)
+        w, ws = weight(k, 200, k, e8)
+        y = ops.fp8_matmul(q, s, w, ws, out_dtype=torch.float32)
+        check_product(y, deq64(q, s, False), deq64(w, ws, True).t(), k, f"m {m}")
+
+
+@pytest.mark.parametrize("e8", [True, False])
+@pytest.mark.parametrize("n,k", [(4096, 1536), (4100, 1040), (2304, 4096), (8192, 100)])
+def test_fp8_matmul_pairs(ops, n, k, e8):
+    """More 128 x 128 tiles than SMs: the CTA pairs, ragged in every size."""
+    m = 148 * 128 * 128 // n // 128 * 128 + 300
+    q, s = ops.act_quant(activations(n, m, k).bfloat16(), 128, "ue8m0" if e8 else None, E8 if e8 else None)
+    for trans in (True, False):
+        nn = n if trans else (n + 15) // 16 * 16
+        w, ws = weight(k, *((nn, k) if trans else (k, nn)), e8)
+        b = deq64(w, ws, True)
+        for out in (torch.bfloat16, torch.float32):
+            y = ops.fp8_matmul(q, s, w, ws, trans_b=trans, out_dtype=out)
+            check_product(y, deq64(q, s, False), b.t() if trans else b, k)
+    ops.fp8_status()
+
+
+def test_offsets_beyond_32_bits(ops):
+    """x, a and y of more than 2^32 bytes: the last rows as computed alone."""
+    rows, k = 1_060_000, 4096
+    x = torch.zeros((rows, k), dtype=torch.bfloat16, device="cuda")
+    x[-200:] = activations(1, 200, k).bfloat16()
+    q, s = ops.act_quant(x, 128, "ue8m0", E8)
+    q1, s1 = ops.act_quant(x[-200:].clone(), 128, "ue8m0", E8)
+    del x
+    assert torch.equal(q[-200:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-200:].float(), s1.float())
+    for n in (64, 2304):                                        # one CTA per tile; pairs
+        w, ws = weight(2, n, k, True)
+        y = ops.fp8_matmul(q, s, w, ws)
+        check_product(y[-200:], deq64(q1, s1, False), deq64(w, ws, True).t(), k)
+        assert (y[:-200] == 0).all()
+        del y
+    ops.fp8_status()
+
+
+def test_large_and_small_products_at_once(ops):
+    """CTA pairs, clusters that split K and the routed layer's kernels on three
+    streams together: clusters whose CTAs wait for one another must all get
+    their tensor memory."""
+    big, bs = weight(1, 2304, 2048, False)
+    w, ws = weight(2, 1024, 4096, True)
+    w2, ws2 = weight(3, 1024, 4096, False)
+    xb, xs = activations(4, 1500, 2048).bfloat16(), activations(5, 100, 4096).bfloat16()
+    want = [ops.fp8_linear(xb, big, bs), ops.fp8_linear(xs, w, ws), ops.fp8_linear(xs, w2, ws2), ops.fp8_linear(xs[:9], w, ws)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    got = [[] for _ in range(4)]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                a, b = ((xb, (big, bs)), (xs, (w, ws)), (xs, (w2, ws2)), (xs[:9], (w, ws)))[i]
+                got[i].append(ops.fp8_linear(a, *b))
+    torch.cuda.synchronize()
+    ops.fp8_status()
+    for i in range(4):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_first_call_of_a_process_in_a_capture(ops):
+    """Nothing has to run before a capture: kernels load and set up inside it."""
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    code = textwrap.dedent("""
+        import torch
+        from dsv4_plugin import ops
+        x = torch.randn(20, 512, device="cuda").bfloat16()
+        w = torch.ones(256, 512, device="cuda").to(torch.float8_e4m3fn)
+        ws = torch.ones(2, 4, device="cuda")
+        lg = torch.randn(20, 16, device="cuda")
+        idx = torch.zeros(20, 2, dtype=torch.int32, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.fp8_linear(x, w, ws)
+            loss, counts = ops.balance_loss(lg, idx, "softmax")
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ops.fp8_linear(x, w, ws)) and int(counts[0]) == 40
+        assert torch.equal(loss, ops.balance_loss(lg, idx, "softmax")[0])
+        print("captured")
+    """)
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join(sys.path))
+    r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
 def test_fp8_matmul_empty(ops):
     w, ws = weight(1, 64, 128, True)
     q, s = ops.act_quant(activations(1, 4, 128), 128, "ue8m0", E8)
