@@ -29,6 +29,10 @@ struct DeviceScope {
     if (cudaGetDevice(&cur) != cudaSuccess) cur = -1;
     if (int rc = bind_device_of(ptr, &device)) return rc;
     if (cur >= 0 && cur != device) prev = cur;
+    // also where the device is the current one: a thread's first call has no
+    // context yet, and encoding a tensor map needs one
+    const cudaError_t e = cudaSetDevice(device);
+    if (e != cudaSuccess) return fail(DSV4_ECUDA, std::string("cudaSetDevice: ") + cudaGetErrorString(e));
     return DSV4_OK;
   }
   ~DeviceScope() {

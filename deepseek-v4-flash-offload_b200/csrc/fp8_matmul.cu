@@ -26,6 +26,7 @@
 
 #include "capi_internal.h"
 #include "common.cuh"
+#include "fp8_quant.cuh"
 
 namespace dsv4 {
 namespace {
@@ -35,6 +36,7 @@ constexpr int F_BM = 128;              // of N (weight rows) per CTA
 constexpr int F_GROUP = 4;             // k-tiles per scale group
 constexpr int F_SLOTS = 4;             // scale groups in flight
 constexpr int F_EPI_WARP0 = 4;
+constexpr int F_MAX_SMEM = 227 * 1024;        // a CTA's opt-in limit
 constexpr int64_t F_MAX_M = 65535LL * 128;   // grid y, in tiles of 128 rows
 
 // Set by a kernel whose bounded wait ran out; read by dsv4_fp8_status.
@@ -49,6 +51,9 @@ struct Fp8Params {
   int kb;              // scale blocks along K = k-tiles
   int vec;             // access width of a row of `as` (scale_vec)
   int out_f32;         // y is fp32, else bf16
+  // rows to quantise (FUSE): bf16 on 16 bytes, K a multiple of 8
+  const uint16_t* x;
+  int64_t ldx, K;
   int vec_y;           // rows of y take vector stores
 };
 
@@ -286,8 +291,12 @@ __device__ __forceinline__ void scale_row(const float* p, int kt, int kb, int ve
 // the tile over the others' shared memory, in rank order.
 //   warp 0: TMA producer, warp 1: MMA issuer, warp 2: scales, warp 3: TMEM
 //   warps 4..: epilogue, 32 of N each (lane = weight row, columns = rows of a)
+// FUSE (a linear layer on up to 64 rows): a's tiles are not loaded but made
+// from the bf16 rows by further warps, a half warp per row and k-tile, codes
+// and scales as act_quant gives them.  One launch instead of two; every CTA
+// quantises its share of K again, out of L2.
 // ---------------------------------------------------------------------------
-template <int BN, bool E8>
+template <int BN, bool E8, bool FUSE = false>
 struct FCfg {
   static constexpr int A_BYTES = F_BM * F_BK;
   static constexpr int B_BYTES = BN * F_BK;
@@ -297,7 +306,10 @@ struct FCfg {
   static constexpr int SLOT_BYTES = E8 ? 1024 : F_GROUP * BN * 4;
   static constexpr int EPI_WARPS = BN >= 64 ? 8 : 4;
   static constexpr int COLS = BN / (EPI_WARPS / 4);      // accumulator columns per epilogue warp
-  static constexpr int THREADS = (F_EPI_WARP0 + EPI_WARPS) * 32;
+  static constexpr int QUANT_WARPS = FUSE ? (BN == 64 ? 8 : 4) : 0;
+  static constexpr int QUANT_WARP0 = F_EPI_WARP0 + EPI_WARPS;
+  static constexpr int THREADS = (QUANT_WARP0 + QUANT_WARPS) * 32;
+  static constexpr int RESIDENT = BN <= 32 || (E8 && !FUSE) ? 2 : 1;   // CTAs per SM (registers)
   static constexpr int NACC = E8 ? 1 : 4;
   static constexpr int SF_COL = BN;                      // E8M0: 8 columns of scales, twice
   static constexpr uint32_t TMEM_COLS = E8 ? (BN == 128 ? 256 : (BN == 64 ? 128 : (BN == 32 ? 64 : 32))) : NACC * BN;
@@ -312,11 +324,21 @@ struct FCfg {
   static_assert(SMEM > 76 * 1024 && (TMEM_COLS <= 256 || SMEM > 134 * 1024), "two CTAs share an SM's TMEM");
 };
 
-template <int BN, bool E8, bool A_MN>
-__global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
+// Eight columns of a row of x from column c (zeros past the end of K).
+__device__ __forceinline__ uint4 x_load(const Fp8Params& p, int64_t m, int64_t c) {
+  return m < p.M && c < p.K ? __ldcg(reinterpret_cast<const uint4*>(p.x + m * p.ldx + c)) : make_uint4(0u, 0u, 0u, 0u);
+}
+__device__ __forceinline__ void x_floats(const uint4& o, float (&v)[8]) {
+  const uint32_t d[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = bf16_from_bits((d[j >> 1] >> (16 * (j & 1))) & 0xffffu);
+}
+
+template <int BN, bool E8, bool A_MN, bool FUSE>
+__global__ void __launch_bounds__(FCfg<BN, E8, FUSE>::THREADS, FCfg<BN, E8, FUSE>::RESIDENT)
     fp8_matmul_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                       const Fp8Params p, const int per) {
-  using C = FCfg<BN, E8>;
+  using C = FCfg<BN, E8, FUSE>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* slots = smem + C::STAGES * C::STAGE_BYTES;
@@ -338,11 +360,11 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
   const int ngr = (nkt + F_GROUP - 1) / F_GROUP;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 1 + C::QUANT_WARPS);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < F_SLOTS; ++s) {
-      mbar_init(&sfull[s], 1);
+      mbar_init(&sfull[s], FUSE && !E8 ? C::QUANT_WARPS : 1);
       mbar_init(&sempty[s], E8 ? 1 : C::EPI_WARPS);
     }
     for (int s = 0; s < C::NACC; ++s) {
@@ -353,7 +375,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
     *err = 0;
     fence_barrier_init();
     prefetch_tensormap(&tmW);
-    prefetch_tensormap(&tmX);
+    if constexpr (!FUSE) prefetch_tensormap(&tmX);
   }
   if (warp == 3) {
     tmem_alloc(tmem_holder, C::TMEM_COLS);
@@ -377,10 +399,10 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
       uint8_t* st = smem + s * C::STAGE_BYTES;
       const int k0 = (kbeg + kt) * F_BK;
       if (elect_one()) {
-        mbar_expect_tx(&full[s], C::STAGE_BYTES);
+        mbar_expect_tx(&full[s], FUSE ? C::A_BYTES : C::STAGE_BYTES);
         if constexpr (A_MN) tma_load_2d(st, &tmW, &full[s], n0, k0, pol);
         else tma_load_2d(st, &tmW, &full[s], k0, n0, pol);
-        tma_load_2d(st + C::A_BYTES, &tmX, &full[s], k0, (int)m0, pol);
+        if constexpr (!FUSE) tma_load_2d(st + C::A_BYTES, &tmX, &full[s], k0, (int)m0, pol);
         mbar_arrive(&full[s]);
       }
       __syncwarp();
@@ -414,12 +436,11 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
         const uint32_t id = kt % F_GROUP, sel = id << 30;
         const uint32_t idesc = idesc_mxf8f6f4(BN, false, id, true) | mn;
         if (elect_one()) {
-          if (fresh) {
-            const uint32_t sl = smem_u32(slots + slot * C::SLOT_BYTES);
-            tc_cp_sf(sfa, desc_sf(sl));
-            tc_cp_sf(sfb, desc_sf(sl + 512));
-            tc_commit(&sempty[slot]);
-          }
+          const uint32_t sl = smem_u32(slots + slot * C::SLOT_BYTES);
+          if (fresh) tc_cp_sf(sfa, desc_sf(sl));
+          // FUSE: the bytes of a's words come one k-tile after the other
+          if (FUSE || fresh) tc_cp_sf(sfb, desc_sf(sl + 512));
+          if (FUSE ? kt % F_GROUP == F_GROUP - 1 || kt == nkt - 1 : fresh) tc_commit(&sempty[slot]);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             tc_mma_mxf8f6f4(tmem, dA + A_STEP * j, dB + 2u * j, idesc, (kt | j) != 0 ? 1u : 0u, sfa | sel, sfb | sel);
@@ -457,6 +478,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
       const uint8_t* bs = static_cast<const uint8_t*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n + (int64_t)kbeg * p.bs_k;
       uint32_t cur[ROWS][4], nxt[ROWS][4], wbyte = 0;
       auto load = [&](int kt) {
+        if constexpr (FUSE) return;   // the quantising warps write a's bytes
 #pragma unroll
         for (int j = 0; j < ROWS; ++j) {
           const int64_t m = m0 + lane + 32 * j;
@@ -484,13 +506,13 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
           for (int j = 0; j < 4; ++j) wb[j] = j < ROWS ? cur[j < ROWS ? j : 0][g] : 0x7f7f7f7fu;
           if (gr + g >= F_SLOTS && !(ok = warp_wait(&sempty[slot], (uint32_t)((gr + g) / F_SLOTS - 1) & 1u, err))) break;
           *reinterpret_cast<uint4*>(sl + lane * 16) = make_uint4(wa, wa, wa, wa);
-          *reinterpret_cast<uint4*>(sl + 512 + lane * 16) = make_uint4(wb[0], wb[1], wb[2], wb[3]);
+          if constexpr (!FUSE) *reinterpret_cast<uint4*>(sl + 512 + lane * 16) = make_uint4(wb[0], wb[1], wb[2], wb[3]);
           fence_proxy_async_smem();   // read by tcgen05.cp
           __syncwarp();
           if (lane == 0) mbar_arrive(&sfull[slot]);
         }
       }
-    } else {
+    } else if constexpr (!FUSE) {
       const float* bs = static_cast<const float*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n + (int64_t)kbeg * p.bs_k;
       float cur[ROWS][F_GROUP], nxt[ROWS][F_GROUP], sb = 0.f;
       auto load = [&](int kt) {
@@ -523,6 +545,66 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
         if (lane == 0) mbar_arrive(&sfull[slot]);
       }
     }
+  } else if (FUSE && warp >= C::QUANT_WARP0) {
+    // ------------------------------------------------------------- quantising
+    constexpr int QW = FUSE ? C::QUANT_WARPS : 1, PASS = FUSE ? BN / (2 * QW) : 1;
+    const int hl = lane & 15, row0 = (warp - C::QUANT_WARP0) * 2 + (lane >> 4);   // rows row0 + i * 2 QW
+    const float* bs = E8 ? nullptr
+                         : static_cast<const float*>(p.bs) + (int64_t)(n0 / F_BK) * p.bs_n + (int64_t)kbeg * p.bs_k;
+    uint4 nxt[PASS];
+    float sb = 0.f;
+    auto load = [&](int kt) {
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) nxt[i] = x_load(p, m0 + row0 + i * 2 * QW, (int64_t)(kbeg + kt) * F_BK + hl * 8);
+      if constexpr (!E8) sb = __ldcg(bs + (int64_t)kt * p.bs_k);
+    };
+    load(0);
+    Ring<C::STAGES> ring;
+    for (int kt = 0; kt < nkt; ++kt, ring.next()) {
+      uint2 code[PASS];
+      float sc[PASS];   // E8M0: the exponent byte
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) {
+        float v[8];
+        x_floats(nxt[i], v);
+        const float a = fp8_amax(v);
+        if constexpr (E8) {
+          const int e = scale_exp_448(a);
+          code[i] = fp8_codes_pow2(v, e);
+          sc[i] = __int_as_float(e + 127);
+        } else {
+          code[i] = fp8_codes_fp32(v, a);
+          sc[i] = fp8_scale_fp32(a) * sb;
+        }
+      }
+      if (kt + 1 < nkt) load(kt + 1);
+      const int gr = kt / F_GROUP, slot = E8 ? gr % F_SLOTS : kt % F_SLOTS;
+      if (kt >= C::STAGES && !warp_wait(&empty[ring.s], ring.ph ^ 1u, err)) break;
+      if constexpr (E8) {
+        if (kt % F_GROUP == 0 && gr >= F_SLOTS && !warp_wait(&sempty[slot], (uint32_t)(gr / F_SLOTS - 1) & 1u, err)) break;
+      } else {
+        if (kt >= F_SLOTS && !warp_wait(&sempty[slot], (uint32_t)(kt / F_SLOTS - 1) & 1u, err)) break;
+      }
+      uint8_t* tile = smem + ring.s * C::STAGE_BYTES + C::A_BYTES;
+      uint8_t* sl = slots + slot * C::SLOT_BYTES;
+#pragma unroll
+      for (int i = 0; i < PASS; ++i) {
+        // rows of 128 bytes, 16-byte units swizzled by row as TMA would
+        const int r = row0 + i * 2 * QW;
+        *reinterpret_cast<uint2*>(tile + r * 128 + (((hl >> 1) ^ (r & 7)) << 4) + (hl & 1) * 8) = code[i];
+        if (hl == 0) {
+          if constexpr (E8) sl[512 + (r & 31) * 16 + (r >> 5) * 4 + kt % F_GROUP] = (uint8_t)__float_as_int(sc[i]);
+          else reinterpret_cast<float*>(sl)[r] = sc[i];
+        }
+      }
+      fence_proxy_async_smem();   // read by the tensor cores
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (!E8) mbar_arrive(&sfull[slot]);
+        mbar_arrive(&full[ring.s]);
+      }
+    }
+    __syncwarp();
   } else if (warp >= F_EPI_WARP0) {
     // -------------------------------------------------------------- epilogue
     const int q = warp & 3, c0 = ((warp - F_EPI_WARP0) >> 2) * C::COLS;
@@ -547,8 +629,10 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
       bool ok = true;
       Ring<C::STAGES> ring;
       for (int kt = 0; kt < nkt; ++kt, ring.next()) {
-        const int ab = kt % C::NACC, gr = kt / F_GROUP, slot = gr % F_SLOTS;
-        if (kt % F_GROUP == 0 && !(ok = warp_wait(&sfull[slot], (uint32_t)(gr / F_SLOTS) & 1u, err))) break;
+        // a slot holds the scales of four k-tiles; FUSE: of one
+        constexpr int SPAN = FUSE ? 1 : F_GROUP;
+        const int ab = kt % C::NACC, gr = kt / SPAN, slot = gr % F_SLOTS;
+        if (kt % SPAN == 0 && !(ok = warp_wait(&sfull[slot], (uint32_t)(gr / F_SLOTS) & 1u, err))) break;
         if (!(ok = warp_wait(&empty[ring.s], ring.ph, err))) break;
         tc_fence_after();
         float v[C::COLS];
@@ -558,7 +642,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&accempty[ab]);
-        const float* f = reinterpret_cast<const float*>(slots + slot * C::SLOT_BYTES) + (kt % F_GROUP) * BN + c0;
+        const float* f = reinterpret_cast<const float*>(slots + slot * C::SLOT_BYTES) + (kt % SPAN) * BN + c0;
 #pragma unroll
         for (int c = 0; c < C::COLS; c += 4) {
           const float4 s = *reinterpret_cast<const float4*>(f + c);
@@ -568,7 +652,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8>::THREADS, E8 ? 2 : 1)
           acc[c + 3] = fmaf(v[c + 3], s.w, acc[c + 3]);
         }
         __syncwarp();
-        if (lane == 0 && (kt % F_GROUP == F_GROUP - 1 || kt == nkt - 1)) mbar_arrive(&sempty[slot]);
+        if (lane == 0 && (kt % SPAN == SPAN - 1 || kt == nkt - 1)) mbar_arrive(&sempty[slot]);
       }
       // the last accumulator is full: no MMA reads the ring any more
       if (ok) {
@@ -1088,6 +1172,9 @@ int sm_count(int dev) {
     known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
+// k-tiles per CTA of a cluster of `want`: a multiple of four, a word of E8M0 scales.
+int k_share(int kb, int want) { return ((kb + want - 1) / want + 3) / 4 * 4; }
+
 template <typename K, typename... Args>
 int launch_cluster(K k, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg = {};
@@ -1108,21 +1195,58 @@ int launch_cluster(K k, dim3 grid, int threads, int smem, dim3 cluster, cudaStre
   return DSV4_OK;
 }
 
-template <int BN, bool E8, bool A_MN>
-int launch_small(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int per, int dev, cudaStream_t st) {
-  using C = FCfg<BN, E8>;
-  static std::atomic<uint64_t> done{0};
-  if (int rc = prepare_kernel(fp8_matmul_kernel<BN, E8, A_MN>, C::SMEM, 0, dev, done)) return rc;
-  const unsigned split = (unsigned)((p.kb + per - 1) / per);
-  const dim3 grid((unsigned)((p.N + F_BM - 1) / F_BM), (unsigned)((p.M + BN - 1) / BN), split);
-  return launch_cluster(fp8_matmul_kernel<BN, E8, A_MN>, grid, C::THREADS, C::SMEM, dim3(1, 1, split), st, tw, tx, p,
-                        per);
+// The largest number of CTAs per cluster, up to `want`, with which all `tiles`
+// clusters are on the GPU at once, `resident` CTAs per SM.  (The CTAs of a
+// cluster share a GPC: at one CTA per SM, 15 clusters of 8 fit 148 SMs, and the
+// 16th doubled the time of 64 x 2048 x 4096 with fp32 scales, 7.5 to 12 us.)
+// The occupancy query answers for one CTA per SM: it is asked with the largest
+// shared memory.
+template <typename K>
+int fitting_cluster(K k, int threads, int resident, int64_t tiles, int want, int dev, std::atomic<int> (&known)[9]) {
+  for (; want > 1; --want) {
+    int n = dev == 0 ? known[want].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1, 1, (unsigned)want);
+      cfg.blockDim = dim3(threads);
+      cfg.dynamicSmemBytes = F_MAX_SMEM;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = (unsigned)want;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        n = 0;
+      }
+      if (n == 0) n = -1;
+      if (dev == 0) known[want].store(n, std::memory_order_relaxed);
+    }
+    if ((int64_t)n * resident >= tiles) break;
+  }
+  return want;
 }
-template <int BN>
-int launch_small(bool e8, bool a_mn, const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int per, int dev,
-                 cudaStream_t st) {
-  if (e8) return a_mn ? launch_small<BN, true, true>(tw, tx, p, per, dev, st) : launch_small<BN, true, false>(tw, tx, p, per, dev, st);
-  return a_mn ? launch_small<BN, false, true>(tw, tx, p, per, dev, st) : launch_small<BN, false, false>(tw, tx, p, per, dev, st);
+template <int BN, bool E8, bool A_MN, bool FUSE>
+int launch_small(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int want, int dev, cudaStream_t st) {
+  using C = FCfg<BN, E8, FUSE>;
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> fits[9];
+  auto k = fp8_matmul_kernel<BN, E8, A_MN, FUSE>;
+  if (int rc = prepare_kernel(k, F_MAX_SMEM, 0, dev, done)) return rc;
+  const int64_t nt = (p.N + F_BM - 1) / F_BM, mt = (p.M + BN - 1) / BN;
+  want = fitting_cluster(k, C::THREADS, C::RESIDENT, nt * mt, want, dev, fits);
+  const int per = k_share(p.kb, want);
+  const unsigned split = (unsigned)((p.kb + per - 1) / per);
+  return launch_cluster(k, dim3((unsigned)nt, (unsigned)mt, split), C::THREADS, C::SMEM, dim3(1, 1, split), st, tw, tx,
+                        p, per);
+}
+template <int BN, bool FUSE>
+int launch_small(bool e8, bool a_mn, const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int want,
+                 int dev, cudaStream_t st) {
+  if (e8) return a_mn ? launch_small<BN, true, true, FUSE>(tw, tx, p, want, dev, st) : launch_small<BN, true, false, FUSE>(tw, tx, p, want, dev, st);
+  return a_mn ? launch_small<BN, false, true, FUSE>(tw, tx, p, want, dev, st) : launch_small<BN, false, false, FUSE>(tw, tx, p, want, dev, st);
 }
 template <bool E8, bool B_MN>
 int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, int sms, int dev, cudaStream_t st) {
@@ -1139,7 +1263,7 @@ int launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p
 struct Fp8Shape {
   bool pair;
   int bn;     // rows of a per CTA's load
-  int per;    // k-tiles per CTA of a cluster that splits K
+  int split;  // CTAs that share K
 };
 // Few rows while the 128 x 128 tiles fit the SMs once: the cluster size then
 // fills the SMs with shares of K.  Measured (us, few rows | pairs), E8M0:
@@ -1147,18 +1271,22 @@ struct Fp8Shape {
 // 1024 x 4096 x 4096 (256 tiles): 23.1 | 18.5, 2048^3: 14.6 | 12.7; fp32
 // scales: 8.1 | 23.8, 12.2 | 14.5, 35.9 | 24.7, 22.9 | 16.0.  Up to 128 of N a
 // pair's 256-wide tile would be half empty.
-Fp8Shape fp8_shape(int64_t m, int64_t n, int kb, int sms) {
+Fp8Shape fp8_shape(int64_t m, int64_t n, int sms) {
   Fp8Shape c = {};
   c.bn = m <= 16 ? 16 : (m <= 32 ? 32 : (m <= 64 ? 64 : 128));
   const int64_t tiles = ((n + F_BM - 1) / F_BM) * ((m + c.bn - 1) / c.bn);
   c.pair = n > 128 && m > 128 && tiles > sms;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(8, sms / tiles));
-  // a multiple of four k-tiles each: a word of E8M0 scales
-  c.per = (int)(((kb + want - 1) / want + 3) / 4 * 4);
+  c.split = (int)std::max<int64_t>(1, std::min<int64_t>(8, sms / tiles));
   return c;
 }
 
 }  // namespace
+
+static int weight_map(CUtensorMap* m, const uint8_t* b, int64_t ldb, bool trans_b, int64_t n, int64_t k) {
+  const uint64_t d[2] = {(uint64_t)(trans_b ? k : n), (uint64_t)(trans_b ? n : k)}, s[1] = {(uint64_t)ldb};
+  const uint32_t box[2] = {128, 128};
+  return make_map(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)b, d, s, box, "fp8 weight");
+}
 
 static int fp8_matmul_run(const uint8_t* a, int64_t lda, const void* as, const uint8_t* b, int64_t ldb, const void* bs,
                           int scale_type, bool trans_b, int64_t m, int64_t n, int64_t k, void* y, int64_t ldy,
@@ -1167,27 +1295,65 @@ static int fp8_matmul_run(const uint8_t* a, int64_t lda, const void* as, const u
   const bool e8 = scale_type == DSV4_SCALE_E8M0, f32 = out_dtype == DSV4_DT_FP32;
   const int sms = sm_count(dev);
   if (sms <= 0) return fail(DSV4_ECUDA, "fp8_matmul: no SM count");
-  const Fp8Shape c = fp8_shape(m, n, (int)kb, sms);
+  const Fp8Shape c = fp8_shape(m, n, sms);
+  Fp8Params p = {};
+  p.as = as, p.bs = bs, p.bs_k = trans_b ? 1 : nb, p.bs_n = trans_b ? kb : 1;
+  p.y = y, p.ldy = ldy, p.M = m, p.N = n, p.kb = (int)kb;
+  p.vec = scale_vec(as, (int)kb, e8);
+  p.out_f32 = f32;
   // 16-byte stores of the pair kernel, four elements of the other
   const int al = c.pair ? 16 : (f32 ? 16 : 8);
-  Fp8Params p{as, bs, trans_b ? 1 : nb, trans_b ? kb : 1, y, ldy, m, n, (int)kb, scale_vec(as, (int)kb, e8), f32,
-              (uintptr_t)y % al == 0 && ldy * (f32 ? 4 : 2) % al == 0};
+  p.vec_y = (uintptr_t)y % al == 0 && ldy * (f32 ? 4 : 2) % al == 0;
   CUtensorMap tw, tx;
-  const uint64_t dw[2] = {(uint64_t)(trans_b ? k : n), (uint64_t)(trans_b ? n : k)}, sw[1] = {(uint64_t)ldb};
-  const uint32_t bw[2] = {128, 128};
-  if (int rc = make_map(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)b, dw, sw, bw, "fp8_matmul b")) return rc;
+  if (int rc = weight_map(&tw, b, ldb, trans_b, n, k)) return rc;
   const uint64_t dx[2] = {(uint64_t)k, (uint64_t)m}, sx[1] = {(uint64_t)lda};
-  const uint32_t bx[2] = {F_BK, (uint32_t)c.bn};
+  const uint32_t bx[2] = {F_BK, (uint32_t)(c.pair ? 128 : c.bn)};
   if (int rc = make_map(&tx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)a, dx, sx, bx, "fp8_matmul a")) return rc;
   if (c.pair) {
     if (e8) return trans_b ? launch_pair<true, false>(tx, tw, p, sms, dev, st) : launch_pair<true, true>(tx, tw, p, sms, dev, st);
     return trans_b ? launch_pair<false, false>(tx, tw, p, sms, dev, st) : launch_pair<false, true>(tx, tw, p, sms, dev, st);
   }
   switch (c.bn) {
-    case 16: return launch_small<16>(e8, !trans_b, tw, tx, p, c.per, dev, st);
-    case 32: return launch_small<32>(e8, !trans_b, tw, tx, p, c.per, dev, st);
-    case 64: return launch_small<64>(e8, !trans_b, tw, tx, p, c.per, dev, st);
-    default: return launch_small<128>(e8, !trans_b, tw, tx, p, c.per, dev, st);
+    case 16: return launch_small<16, false>(e8, !trans_b, tw, tx, p, c.split, dev, st);
+    case 32: return launch_small<32, false>(e8, !trans_b, tw, tx, p, c.split, dev, st);
+    case 64: return launch_small<64, false>(e8, !trans_b, tw, tx, p, c.split, dev, st);
+    default: return launch_small<128, false>(e8, !trans_b, tw, tx, p, c.split, dev, st);
+  }
+}
+
+// Whether a linear layer quantises its rows in the product's launch.  Every
+// CTA then quantises its share of K again, so that share has to be short: the
+// second launch costs about 2 us, a k-tile 0.15 us (16 rows) to 0.4 us (64
+// rows), more with fp32 scales.  Measured (us, one launch | two; E8M0): 1 x
+// 4096 x 4096: 6.4 | 8.2, 64 x 4096 x 2048 (4 k-tiles): 7.7 | 8.1, 64 x 8192 x
+// 8192 (32 k-tiles): 28 | 17; fp32: 1 x 2048 x 4096: 6.3 | 6.6, 64 x 4096 x
+// 2048: 10.4 | 8.5.
+static bool linear_fuses(const void* x, int x_dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, bool e8, int sms) {
+  if (m > 64 || x_dtype != DSV4_DT_BF16 || k % 8 || (uintptr_t)x % 16 || ldx % 8) return false;
+  const int split = fp8_shape(m, n, sms).split, per = k_share((int)((k + F_BK - 1) / F_BK), split);
+  if (m <= 16) return per <= (e8 ? 8 : 4);
+  // above 32 rows one CTA fits an SM, and few clusters of more than four do
+  return e8 && per <= 4 && (m <= 32 || split <= 4);
+}
+static int fp8_linear_fused(const void* x, int64_t ldx, const uint8_t* w, int64_t ldw, const void* ws,
+                            int scale_type, bool trans_w, int64_t m, int64_t n, int64_t k, void* y, int64_t ldy,
+                            int dev, cudaStream_t st) {
+  const int64_t kb = (k + F_BK - 1) / F_BK, nb = (n + F_BK - 1) / F_BK;
+  const bool e8 = scale_type == DSV4_SCALE_E8M0;
+  const int sms = sm_count(dev);
+  if (sms <= 0) return fail(DSV4_ECUDA, "fp8_linear: no SM count");
+  const Fp8Shape c = fp8_shape(m, n, sms);
+  Fp8Params p = {};
+  p.bs = ws, p.bs_k = trans_w ? 1 : nb, p.bs_n = trans_w ? kb : 1;
+  p.y = y, p.ldy = ldy, p.M = m, p.N = n, p.kb = (int)kb;
+  p.vec_y = (uintptr_t)y % 8 == 0 && ldy % 4 == 0;
+  p.x = static_cast<const uint16_t*>(x), p.ldx = ldx, p.K = k;
+  CUtensorMap tw;
+  if (int rc = weight_map(&tw, w, ldw, trans_w, n, k)) return rc;
+  switch (c.bn) {
+    case 16: return launch_small<16, true>(e8, !trans_w, tw, tw, p, c.split, dev, st);
+    case 32: return launch_small<32, true>(e8, !trans_w, tw, tw, p, c.split, dev, st);
+    default: return launch_small<64, true>(e8, !trans_w, tw, tw, p, c.split, dev, st);
   }
 }
 
@@ -1258,6 +1424,8 @@ extern "C" int dsv4_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, cons
   DeviceScope dev;
   if (int rc = dev.enter(x)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
+  if (linear_fuses(x, x_dtype, ldx, m, n, k, scale_type == DSV4_SCALE_E8M0, sm_count(dev.device)))
+    return fp8_linear_fused(x, ldx, w, ldw, w_scale, scale_type, trans_w != 0, m, n, k, y, ldy, dev.device, st);
   uint8_t* q = static_cast<uint8_t*>(workspace);
   uint8_t* s = q + linear_scale_offset(m, k);
   const int64_t ldq = (k + 15) / 16 * 16;

@@ -1,18 +1,7 @@
 // Activation quantisation with separate outputs: E4M3 codes and one scale per
 // row and 128 columns (act_quant, inplace=False; npu_ops.py:73-104).
 //
-// For a block of 128 columns with a = max(1e-4, max |x|):
-//   power-of-two scales: s = 2^e with the smallest e that gives a <= 448 2^e,
-//     q = e4m3(x 2^-e) (the division is exact, so q has one rounding);
-//   fp32 scales: s = a / 448, q = e4m3(448 x / a).  The quotient is the product
-//     with the block's reciprocal, corrected once by its exact remainder
-//     (Markstein 1990): exact where the real quotient is an fp32 number, else
-//     within 2^-23.  For 16-bit x a quotient is a tie of E4M3 or more than
-//     2^-20 away from one (the significands are short), so q is the nearest
-//     code to the real 448 x / a.  A division per element was the limit: 27.8
-//     us instead of 21.4 for 8192 x 4096 bf16.
-// A NaN stays NaN and leaves its block's scale alone; an infinity takes the
-// largest finite value's scale and saturates.
+// The arithmetic is in fp8_quant.cuh.
 //
 // Bound: HBM, (bytes of x + 1) per element.  A half warp holds a block, eight
 // columns per lane, so a lane loads 16 bytes (two loads for fp32) and stores
@@ -21,6 +10,7 @@
 // lanes.
 #include "capi_internal.h"
 #include "common.cuh"
+#include "fp8_quant.cuh"
 
 #include <cuda_fp16.h>
 
@@ -48,22 +38,6 @@ struct In<DSV4_DT_FP32> {
   using T = float;
   static __device__ __forceinline__ float f(T v) { return v; }
 };
-
-// Smallest e with a <= 448 * 2^e (448 = 1.75 * 2^8), a normal and finite.
-__device__ __forceinline__ int scale_exp_448(float a) {
-  const uint32_t u = __float_as_uint(a);
-  return (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
-}
-
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
-
-// n / d with r = 1 / d rounded to nearest; infinities and NaN as n r.
-__device__ __forceinline__ float quotient(float n, float d, float r) {
-  const float q = n * r;
-  return fabsf(q) < 1e30f ? fmaf(fmaf(-q, d, n), r, q) : q;
-}
 
 // VEC: rows of x start on 16 bytes, rows of q on 8, and cols % 8 == 0.
 template <int DT, int SC, bool VEC>
@@ -103,30 +77,15 @@ __global__ void __launch_bounds__(Q_THREADS)
   }
 #pragma unroll
   for (int i = 0; i < Q_STEPS; ++i) {
-    float a = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(v[i][j]));   // fmaxf drops a NaN
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-    a = fminf(fmaxf(a, 1e-4f), 3.402823466e+38f);
+    const float a = fp8_amax(v[i]);
     const int64_t b = b0 + 2 * i;
-    uint32_t o[2];
+    uint2 o;
     if constexpr (SC == DSV4_SCALE_FP32) {
-      const float den = a * 0.001953125f, rec = __frcp_rn(den);   // a / 512, exact: 448 x / a = (0.875 x) / (a / 512)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t p = e4m3x2(quotient(0.875f * v[i][2 * j], den, rec), quotient(0.875f * v[i][2 * j + 1], den, rec));
-        o[j >> 1] = (j & 1) ? (o[j >> 1] | (p << 16)) : p;
-      }
-      if (hl == 0 && b < nb) static_cast<float*>(scale)[row * nb + b] = __fdiv_rn(a, 448.f);
+      o = fp8_codes_fp32(v[i], a);
+      if (hl == 0 && b < nb) static_cast<float*>(scale)[row * nb + b] = fp8_scale_fp32(a);
     } else {
       const int e = scale_exp_448(a);
-      const float inv = pow2i(-e);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t p = e4m3x2(v[i][2 * j] * inv, v[i][2 * j + 1] * inv);
-        o[j >> 1] = (j & 1) ? (o[j >> 1] | (p << 16)) : p;
-      }
+      o = fp8_codes_pow2(v[i], e);
       if (hl == 0 && b < nb) {
         if constexpr (SC == DSV4_SCALE_E8M0) static_cast<uint8_t*>(scale)[row * nb + b] = (uint8_t)(e + 127);
         else static_cast<float*>(scale)[row * nb + b] = pow2i(e);
@@ -134,11 +93,11 @@ __global__ void __launch_bounds__(Q_THREADS)
     }
     const int64_t c = b * QB + (VEC ? hl * 8 : hl);
     if constexpr (VEC) {
-      if (c < cols) *reinterpret_cast<uint2*>(qr + c) = make_uint2(o[0], o[1]);
+      if (c < cols) *reinterpret_cast<uint2*>(qr + c) = o;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j * 16 < cols) qr[c + j * 16] = (uint8_t)(o[j >> 2] >> (8 * (j & 3)));
+        if (c + j * 16 < cols) qr[c + j * 16] = (uint8_t)((j < 4 ? o.x : o.y) >> (8 * (j & 3)));
     }
   }
 }

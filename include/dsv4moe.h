@@ -139,7 +139,8 @@ int dsv4_fp8_matmul(const uint8_t* a, int64_t lda, const void* a_scale, const ui
  * or fp32, row stride ldx elements) into the workspace with scales of
  * scale_type (DSV4_SCALE_E8M0 or DSV4_SCALE_FP32, the type of w_scale), then
  * dsv4_fp8_matmul with w (trans_w != 0: [n, k], y = x w^T; 0: [k, n], y = x w,
- * the input gradient of the former) into y [m, n] of x's type. */
+ * the input gradient of the former) into y [m, n] of x's type.  A few bf16
+ * rows take one launch; the results are the same. */
 int64_t dsv4_fp8_linear_workspace_bytes(int64_t m, int64_t k, int32_t scale_type);
 int dsv4_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw, const void* w_scale,
                     int32_t scale_type, int32_t trans_w, int64_t m, int64_t n, int64_t k, void* y, int64_t ldy,

@@ -287,6 +287,26 @@ def test_large_and_small_products_at_once(ops):
         assert all(torch.equal(y, want[i]) for y in got[i])
 
 
+def test_first_call_of_a_thread(ops):
+    """A thread without a CUDA context of its own yet, as autograd's are."""
+    import threading
+    w, ws = weight(1, 256, 512, True)
+    q, s = ops.act_quant(activations(1, 8, 512), 128, "ue8m0", E8)
+    x = activations(2, 8, 512).bfloat16()
+    want = [ops.fp8_matmul(q, s, w, ws), ops.fp8_linear(x, w, ws)]
+    got = [None, None]
+
+    def run(i):
+        got[i] = ops.fp8_matmul(q, s, w, ws) if i == 0 else ops.fp8_linear(x, w, ws)
+        torch.cuda.current_stream().synchronize()
+
+    for i in range(2):
+        t = threading.Thread(target=run, args=(i,))
+        t.start()
+        t.join()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_first_call_of_a_process_in_a_capture(ops):
     """Nothing has to run before a capture: kernels load and set up inside it."""
     import os
@@ -385,6 +405,30 @@ def test_fp8_linear_and_its_gradient(ops, m, n, k, e8, dtype):
     lost = 2.0 ** -50 / h * ((d64.abs() * ((deq64(qx, sx, False).abs() + h * v.abs()) @ w64.abs().t())).sum(1))
     tol = ((n / 32 + 34) * 2.0 ** -23 + (2.0 ** -8 if dtype == torch.bfloat16 else 0)) * mag + lost
     assert ((up - dn) / (2 * h) - slope).abs().le(tol).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("e8", [True, False])
+@pytest.mark.parametrize("m,n,k", [(1, 2048, 4096), (2, 130, 1), (5, 100, 333), (16, 256, 1000), (17, 4096, 2048),
+                                   (33, 127, 3584), (64, 1001, 4104), (64, 20000, 512), (65, 300, 1024), (400, 256, 520)])
+def test_fp8_linear_is_its_parts(ops, m, n, k, e8, dtype):
+    """Quantisation and product in one launch (up to 64 rows) or two: the bits
+    of act_quant and fp8_matmul called one after the other, forward and for
+    the gradient; values with a NaN, an infinity and a row of zeros."""
+    w, ws = weight(n + k, n, k, e8)
+    x = activations(m + k, m, k).to(dtype)
+    x[m // 2] = 0
+    if k > 10:
+        x[0, 3], x[-1, 10] = float("nan"), float("inf")
+    dy = activations(m + n, m, n).to(dtype)
+    fmt, sd = ("ue8m0", E8) if e8 else (None, None)
+    xr = x.clone().requires_grad_(True)
+    y = ops.fp8_linear(xr, w, ws)
+    dx, = torch.autograd.grad(y, xr, dy)
+    same = lambda a, b: torch.equal(torch.nan_to_num(a, nan=12345.0), torch.nan_to_num(b, nan=12345.0))  # noqa: E731
+    assert same(y.detach(), ops.fp8_matmul(*ops.act_quant(x, 128, fmt, sd), w, ws, out_dtype=dtype))
+    assert same(dx, ops.fp8_matmul(*ops.act_quant(dy, 128, fmt, sd), w, ws, trans_b=False, out_dtype=dtype))
+    ops.fp8_status()
 
 
 def test_fp8_linear_shapes(ops):

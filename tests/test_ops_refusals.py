@@ -144,6 +144,27 @@ def test_fp8_matmul_entry_refuses():
     assert L.dsv4_fp8_matmul(None, 256, None, None, 256, None, 0, 1, 0, 16, 256, None, 16, 0, None) == 0
 
 
+def test_fp8_linear_entry_refuses():
+    L = _lib.lib()
+    assert L.dsv4_fp8_linear_workspace_bytes(100, 250, 0) == 100 * (256 + 2)
+    assert L.dsv4_fp8_linear_workspace_bytes(100, 256, 1) == 100 * (256 + 8)
+    for bad in ((-1, 256, 0), (4, 0, 0), (4, 256, 2), (1 << 40, 256, 0)):
+        assert L.dsv4_fp8_linear_workspace_bytes(*bad) == _lib.DSV4_EINVAL
+
+    def call(x=P, dt=0, ldx=256, w=P, ldw=256, sw=P, kind=0, tw=1, m=100, n=16, k=256, y=P, ldy=16, ws=P, nb=1 << 20):
+        return refused("dsv4_fp8_linear", x, dt, ldx, w, ldw, sw, kind, tw, m, n, k, y, ldy, ws, nb, None)
+
+    for name in ("x", "w", "sw", "y", "ws"):
+        assert "null" in call(**{name: None})
+    assert "bf16" in call(dt=1) and "E8M0" in call(kind=2) and "k > 0" in call(k=0)
+    assert "stride" in call(ldx=255) and "stride" in call(ldw=240) and "stride" in call(ldy=15)
+    assert "stride" in call(tw=0, n=272, ldy=272)
+    assert "16 bytes" in call(w=P + 8) and "16 bytes" in call(ldw=264)
+    assert "misaligned" in call(x=P + 1) and "misaligned" in call(y=P + 1) and "misaligned" in call(sw=P + 2, kind=1)
+    assert "workspace" in call(nb=100) and "workspace" in call(ws=P + 8)
+    assert "too large" in call(m=1 << 40)
+
+
 def test_balance_entries_refuse():
     L = _lib.lib()
     big = L.dsv4_balance_workspace_bytes(100, 8, 2)
