@@ -18,8 +18,9 @@
 //   three k-tiles' MMAs, hence four of them.
 //
 // Measured (device, graph replay): 1 x 2048 x 4096 5.0 us, 64 x 4096 x 4096 7.4
-// us, 2048 x 4096 x 4096 28 us, 8192 x 8192 x 4096 200 us (2.75 PFLOP/s) with
-// E8M0 scales, 285 us (1.93 PFLOP/s) with fp32 scales.  Few rows are bound by
+// us, 2048 x 4096 x 4096 29 us, 8192 x 8192 x 4096 206 us (2.67 PFLOP/s) with
+// E8M0 scales, 288 us (1.91 PFLOP/s) with fp32 scales; the same inputs in every
+// replay, so the small ones stay in L2.  Few rows are bound by
 // latency (the weights alone would take 1.3 us of HBM time for the first), many
 // by the tensor cores and L2 (64 B per clock and SM), fp32 scales by the
 // epilogue's multiply-adds.
@@ -160,7 +161,8 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // Arrival that publishes nothing (an accumulator has been read: its values are
-// in registers).  A release at cluster scope here cost 0.6 us per k-tile.
+// in registers).  A release at cluster scope here, and
+// an acquire in the wait for it, cost 1.1 us per k-tile together.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
@@ -731,9 +733,9 @@ __global__ void __launch_bounds__(FCfg<BN, E8, FUSE>::THREADS, FCfg<BN, E8, FUSE
 // E8M0: one accumulator of 256 columns, released as soon as the epilogue has it
 // in registers.  fp32 scales: two of 256 columns, a k-tile each; an epilogue
 // thread has one row of one 128-block of N, so a partial sum takes one
-// multiply-add.  (Four accumulators of 128 columns would hide the hand-over
-// better, but MMAs of 128 columns read a's tile from shared memory twice as
-// often, and that bandwidth is the limit: 1.24 us per k-tile of 256 x 256.)
+// multiply-add.  (Four accumulators of 128 columns, whose MMAs read a's tile
+// from shared memory twice as often, took 0.67 us per k-tile of 256 x 256; two
+// of 256 first took 0.66 and take 0.54 with the waits tested ahead.)
 // ---------------------------------------------------------------------------
 constexpr int L_TM = 256;
 constexpr int L_SF_COL = 256;                    // 12 columns of scales, twice

@@ -76,7 +76,8 @@ def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt: str | None = "u
     ``scale_fmt="ue8m0"``: the smallest power of two that brings the block
     within 448, as ``scale_dtype`` float32 (also None) or float8_e8m0fnu;
     ``scale_fmt=None``: amax / 448 in float32.  amax is at least 1e-4.  A NaN
-    stays NaN and leaves its block's scale alone; an infinity saturates."""
+    stays NaN and leaves its block's scale alone; an infinity saturates.  The
+    result carries no gradient (``fp8_linear`` does)."""
     if block_size != 128 or scale_fmt not in ("ue8m0", None):
         raise NotImplementedError("act_quant provides block_size 128 and scale_fmt 'ue8m0' or None")
     if inplace:
@@ -251,7 +252,9 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
     Differentiable in ``x``: the gradient dy is quantised the same way, along
     N, and multiplied with the same stored weight (the rounding of x is passed
-    through).  The weight is a checkpoint's and gets no gradient."""
+    through).  The weight is a checkpoint's and gets no gradient.  As with
+    torch's own operators, a backward pass is captured into a CUDA graph only
+    while no eager graph of the same leaves is alive."""
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"fp8_linear expects bf16 or fp32, got {x.dtype}")
     _check_fp8_weight(weight, weight_scale)
