@@ -728,6 +728,7 @@ extern "C" int dsv4_balance_forward(const void* logits, int32_t dtype, int64_t n
   DSV4_CHECK_ARG(!bad, bad);
   DSV4_CHECK_ARG(dtype == DSV4_DT_FP32 || dtype == DSV4_DT_BF16, "logits must be fp32 or bf16");
   DSV4_CHECK_ARG(topk >= 1, "topk must be positive");
+  DSV4_CHECK_ARG(n_tokens <= 0x7fffffff / topk, "n_tokens * topk must be below 2^31: picks are counted in 32 bits");
   DSV4_CHECK_ARG(score_func >= DSV4_SCORE_SOFTMAX && score_func <= DSV4_SCORE_SQRTSOFTPLUS, "unknown score function");
   DSV4_CHECK_ARG(seq_offsets || n_seqs == 1, "several sequences need their offsets");
   DSV4_CHECK_ARG(loss && counts && workspace && (n_tokens == 0 || (logits && indices)), "null pointer");

@@ -399,7 +399,7 @@ def balance_loss(logits: torch.Tensor, indices: torch.Tensor, score_func: str = 
     ``seq_offsets``, which ``parallel_ep.balanced_placement`` takes as loads).
 
     ``logits`` [T, E] fp32 or bf16 (E <= 1024), ``indices`` [T, k] the
-    router's picks (``route_topk``; -1 = empty).  ``seq_offsets`` [S + 1]
+    router's picks (``route_topk``; -1 = empty; T k < 2^31).  ``seq_offsets`` [S + 1]
     (integer, ascending, on the device) packs S sequences: rows o[s] ..
     o[s+1]-1 are sequence s.  A row without a pick and a row outside the
     sequences are padding: they do not count and their gradient is 0.  With p

@@ -165,7 +165,8 @@ int dsv4_fp8_status(int32_t device, void* stream);
  * NaN or an infinite score makes the loss and its row's gradient NaN.  Picks
  * outside [-1, n_experts) are skipped, and like offsets that descend or
  * leave [0, n_tokens] they set DSV4_EINVAL in *status (device word, may be
- * NULL).  logits are fp32 or bf16 [n_tokens, n_experts], n_experts <= 1024.
+ * NULL).  logits are fp32 or bf16 [n_tokens, n_experts], n_experts <= 1024,
+ * n_tokens * topk < 2^31.
  * The forward leaves in the workspace what the backward reads: dlogits (type
  * of the logits, every row written, rows that do not count as zeros) =
  * *grad_loss (device) times the gradient with the counts held constant.

@@ -191,3 +191,11 @@ def test_balance_entries_refuse():
     for name in ("lg", "up", "out", "ws"):
         assert "null" in bwd(**{name: None})
     assert "fp32" in bwd(dt=1) and "score" in bwd(score=-1) and "workspace" in bwd(nb=16)
+
+
+@pytest.mark.parametrize("t,k", [(1 << 30, 2), (1 << 28, 8), ((1 << 31) - 1, 2)])
+def test_balance_refuses_more_picks_than_it_can_count(t, k):
+    """The picks of a sequence are counted in 32 bits."""
+    nb = _lib.lib().dsv4_balance_workspace_bytes(t, 8, 1)
+    assert "picks" in refused("dsv4_balance_forward", P, _lib.DT_FP32, t, 8, P, k, None, 1, 0, C.c_float(1.0), P, P, P,
+                              nb, None, None)
