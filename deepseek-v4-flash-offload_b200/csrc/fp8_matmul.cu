@@ -161,8 +161,8 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
 // Arrival that publishes nothing (an accumulator has been read: its values are
-// in registers).  A release at cluster scope here, and
-// an acquire in the wait for it, cost 1.1 us per k-tile together.
+// in registers).  A release at cluster scope here, and an acquire in the wait
+// for it, cost 1.1 us per k-tile together.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
@@ -329,7 +329,8 @@ struct FCfg {
   // The CTAs of a cluster wait for one another, so a CTA that is resident must
   // get its TMEM without waiting for another resident one: at most two of
   // these CTAs fit an SM (shared memory), and either both take at most half
-  // of the 512 columns or one leaves no room for the other.
+  // of the 512 columns or one leaves no room for the other.  (The routed
+  // layer's kernels with TMEM take 176 KB or more: none shares an SM with these.)
   static_assert(SMEM > 76 * 1024 && (TMEM_COLS <= 256 || SMEM > 134 * 1024), "two CTAs share an SM's TMEM");
 };
 

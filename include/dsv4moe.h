@@ -161,7 +161,8 @@ int dsv4_fp8_status(int32_t device, void* stream);
  * tokens of sequence s, f[s, e] = c[s, e] * n_experts / sum_e c[s, e]:
  *   loss = alpha * mean over sequences with tokens of
  *          sum_e f[s, e] * (1 / n[s]) * sum_t p[t, e];
- * counts [n_seqs, n_experts] = c.  A row whose scores are all 0 has p = 0; a
+ * counts [n_seqs, n_experts] = c.  A row whose scores are all 0 has p = 0 (a
+ * sigmoid below 2^-126, the smallest normal fp32 number, counts as 0); a
  * NaN or an infinite score makes the loss and its row's gradient NaN.  Picks
  * outside [-1, n_experts) are skipped, and like offsets that descend or
  * leave [0, n_tokens] they set DSV4_EINVAL in *status (device word, may be
