@@ -31,18 +31,12 @@ E8 = torch.float8_e8m0fnu
 DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 
 
-_loaded = None
-
-
 def _ops():
-    """The framework's operators, imported once as a user's program does."""
-    global _loaded
-    if _loaded is None:
-        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                                        "deepseek-v4-flash-offload_b200"))
-        from dsv4_plugin import ops
-        _loaded = ops
-    return _loaded
+    here = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "deepseek-v4-flash-offload_b200")
+    if here not in sys.path:
+        sys.path.insert(0, here)
+    from dsv4_plugin import ops
+    return ops
 
 
 # -- cases ---------------------------------------------------------------------
