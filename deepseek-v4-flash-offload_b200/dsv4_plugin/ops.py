@@ -356,11 +356,25 @@ def moe_align(indices: torch.Tensor, n_experts: int) -> dict:
     return out
 
 
+class _DifferentiatedOnce(torch.autograd.Function):
+    """A gradient computed from ``inputs`` outside autograd: differentiating
+    it raises (an untracked result would only leave the term out)."""
+
+    @staticmethod
+    def forward(ctx, what, grad, *inputs):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.what} is differentiable once")
+
+
 class _BalanceLoss(torch.autograd.Function):
+    # logits: contiguous
     @staticmethod
     def forward(ctx, logits, indices, offsets, n_seqs, score, alpha, status):
         t, e = logits.shape
-        logits = logits.contiguous()
         nb = lib().dsv4_balance_workspace_bytes(t, e, n_seqs)
         ws = logits.new_empty(nb, dtype=torch.uint8)
         loss = logits.new_empty((), dtype=torch.float32)
@@ -379,8 +393,6 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, grad_loss, _):
         if grad_loss is None:
             return None, None, None, None, None, None, None
-        if grad_loss.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("balance_loss is differentiable once")
         logits, ws = ctx.saved_tensors
         n_seqs, score, alpha = ctx.args
         t, e = logits.shape
@@ -389,13 +401,15 @@ class _BalanceLoss(torch.autograd.Function):
         check(lib().dsv4_balance_backward(logits.data_ptr(), _DT[logits.dtype], t, e, n_seqs, score, alpha,
                                           up.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel(),
                                           _stream(logits.device)))
+        if torch.is_grad_enabled():           # create_graph
+            out = _DifferentiatedOnce.apply("balance_loss", out, logits, up)
         return out, None, None, None, None, None, None
 
 
 def balance_loss(logits: torch.Tensor, indices: torch.Tensor, score_func: str = "sqrtsoftplus", alpha: float = 1.0,
                  seq_offsets: torch.Tensor | None = None, status: torch.Tensor | None = None):
-    """Load balance loss of a router (float32 scalar, differentiable in
-    ``logits``) and the picks per expert (int32 [E], or [S, E] with
+    """Load balance loss of a router (float32 scalar, differentiable once in
+    ``logits``: a second derivative raises) and the picks per expert (int32 [E], or [S, E] with
     ``seq_offsets``, which ``parallel_ep.balanced_placement`` takes as loads).
 
     ``logits`` [T, E] fp32 or bf16 (E <= 1024), ``indices`` [T, k] the
@@ -434,8 +448,8 @@ def balance_loss(logits: torch.Tensor, indices: torch.Tensor, score_func: str = 
         if seq_offsets.dtype == torch.int64:
             seq_offsets = seq_offsets.clamp(-1, 0x7fffffff).to(torch.int32)
         seq_offsets = seq_offsets.contiguous()
-    loss, counts = _BalanceLoss.apply(logits, indices.contiguous(), seq_offsets, n_seqs, SCORE_FUNCS[score_func],
-                                      float(alpha), status)
+    loss, counts = _BalanceLoss.apply(logits.contiguous(), indices.contiguous(), seq_offsets, n_seqs,
+                                      SCORE_FUNCS[score_func], float(alpha), status)
     return loss, counts
 
 
