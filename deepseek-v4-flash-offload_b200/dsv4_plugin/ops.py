@@ -21,6 +21,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import (DT_BF16, DT_FP16, DT_FP32, PROFILES, ROWS_BF16, ROWS_FP8, ROWS_MXFP4,  # noqa: F401
                    SCALE_E8M0, SCALE_FP32, SCALE_FP32_POW2, SCORE_FUNCS, check, lib)
@@ -244,6 +245,12 @@ class _Fp8Linear(torch.autograd.Function):
         return _fp8_linear_call(dy, w, ws, False), None, None
 
 
+def _has_tangent(*ts) -> bool:
+    """A tensor is a forward-mode dual one (outside a dual level none is)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and \
+        any(forward_ad.unpack_dual(t).tangent is not None for t in ts)
+
+
 def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor) -> torch.Tensor:
     """Linear layer on a frozen FP8 weight [N, K] with one scale per 128 x 128
     block: ``act_quant(x)`` (power-of-two scales for an E8M0 ``weight_scale``,
@@ -252,7 +259,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
     Differentiable in ``x``: the gradient dy is quantised the same way, along
     N, and multiplied with the same stored weight (the rounding of x is passed
-    through).  The weight is a checkpoint's and gets no gradient.  As with
+    through).  The weight is a checkpoint's and gets no gradient.  Forward-mode
+    tangents are refused.  As with
     torch's own operators, a backward pass is captured into a CUDA graph only
     while no eager graph of the same leaves is alive."""
     if x.dtype not in (torch.bfloat16, torch.float32):
@@ -264,8 +272,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
         raise ValueError(f"x {tuple(x.shape)} does not match the weight {tuple(weight.shape)}")
     _is_e8m0(weight_scale)
     _same_device(x, weight, weight_scale)
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Fp8Linear.apply(x, weight, weight_scale)
+    if (x.requires_grad and torch.is_grad_enabled()) or _has_tangent(x, weight, weight_scale):
+        return _Fp8Linear.apply(x, weight, weight_scale)      # which refuses a tangent
     return _fp8_linear_call(x, weight, weight_scale, True)
 
 

@@ -51,3 +51,22 @@ def test_balance_loss_first_derivative_under_create_graph(strided):
     loss, _ = ops.balance_loss(logits, idx)
     loss.backward()
     assert logits.grad.shape == logits.shape and not logits.grad.requires_grad
+
+
+def fp8_layer(n=16, k=128):
+    w = torch.zeros(n, k, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    return w, torch.ones((n + 127) // 128, 1)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_fp8_linear_refuses_forward_mode(grad):
+    """A tangent is refused, not dropped, whether or not x requires a gradient."""
+    from torch.autograd import forward_ad
+    w, s = fp8_layer()
+    x = torch.zeros(3, 128, requires_grad=grad)
+    with forward_ad.dual_level():
+        assert ops.fp8_linear(x, w, s).shape == (3, 16)        # no tangent: as outside
+        with pytest.raises(RuntimeError, match="forward"):
+            ops.fp8_linear(forward_ad.make_dual(x, torch.ones(3, 128)), w, s)
+        with pytest.raises(RuntimeError, match="forward"):
+            ops.fp8_linear(x, w, forward_ad.make_dual(s, torch.ones_like(s)))
