@@ -214,6 +214,8 @@ def _fp8_linear_call(x: torch.Tensor, w: torch.Tensor, ws: torch.Tensor, trans: 
     """act_quant(x) times w (trans: w.T) -> x's type; scales of ws's type."""
     k = x.shape[-1]
     n = w.shape[0 if trans else 1]
+    if k == 0:      # the gradient of a layer without outputs
+        return x.new_zeros((*x.shape[:-1], n))
     y = x.new_empty((*x.shape[:-1], n))
     m = y.numel() // n if n else 0
     if m == 0:

@@ -70,3 +70,16 @@ def test_fp8_linear_refuses_forward_mode(grad):
             ops.fp8_linear(forward_ad.make_dual(x, torch.ones(3, 128)), w, s)
         with pytest.raises(RuntimeError, match="forward"):
             ops.fp8_linear(x, w, forward_ad.make_dual(s, torch.ones_like(s)))
+
+
+@pytest.mark.parametrize("shape", [(3, 128), (2, 3, 128), (0, 128)])
+def test_fp8_linear_with_an_empty_weight(shape):
+    """No output columns: the gradient of x is a sum over nothing."""
+    w, s = fp8_layer(0)
+    x = torch.ones(shape, requires_grad=True)
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(ops, "lib", lambda: pytest.fail("an empty product calls no kernel"))
+        y = ops.fp8_linear(x, w, s)
+        assert y.shape == (*shape[:-1], 0)
+        dx, = torch.autograd.grad(y, x, torch.zeros_like(y))
+    assert dx.shape == x.shape and dx.dtype == x.dtype and not dx.any()
