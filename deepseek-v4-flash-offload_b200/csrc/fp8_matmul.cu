@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(FCfg<BN, E8, FUSE>::THREADS, FCfg<BN, E8, FUSE
           code[i] = fp8_codes_pow2(v, e);
           sc[i] = __int_as_float(e + 127);
         } else {
-          code[i] = fp8_codes_fp32(v, a);
+          code[i] = fp8_codes_fp32<false>(v, a);
           sc[i] = fp8_scale_fp32(a) * sb;
         }
       }

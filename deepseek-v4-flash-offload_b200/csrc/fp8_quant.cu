@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(Q_THREADS)
     const int64_t b = b0 + 2 * i;
     uint2 o;
     if constexpr (SC == DSV4_SCALE_FP32) {
-      o = fp8_codes_fp32(v[i], a);
+      o = fp8_codes_fp32<DT == DSV4_DT_FP32>(v[i], a);
       if (hl == 0 && b < nb) static_cast<float*>(scale)[row * nb + b] = fp8_scale_fp32(a);
     } else {
       const int e = scale_exp_448(a);

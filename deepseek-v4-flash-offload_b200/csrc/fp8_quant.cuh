@@ -5,13 +5,15 @@
 // With a = max(1e-4, max |x|) of the block:
 //   power-of-two scales: s = 2^e with the smallest e that gives a <= 448 2^e,
 //     q = e4m3(x 2^-e) (the division is exact, so q has one rounding);
-//   fp32 scales: s = a / 448, q = e4m3(448 x / a).  The quotient is the product
-//     with the block's reciprocal, corrected once by its exact remainder
-//     (Markstein 1990): exact where the real quotient is an fp32 number, else
-//     within 2^-23.  For 16-bit x a quotient is a tie of E4M3 or more than
-//     2^-20 away from one (the significands are short), so q is the nearest
-//     code to the real 448 x / a.  A division per element was the limit: 27.8
-//     us instead of 21.4 for 8192 x 4096 bf16.
+//   fp32 scales: s = a / 448, q = the E4M3 value nearest to the real 448 x / a.
+//     The quotient is the product with the block's reciprocal, corrected once
+//     by its remainder (Markstein 1990), and then less than one step of fp32
+//     from the real one.  For 16-bit x (0.875 x is exact) a quotient is a tie
+//     of E4M3 or more than 2^-20 away from one, so rounding it gives the
+//     nearest code.  For fp32 x the remainder takes in what 0.875 x lost, and
+//     a quotient that comes out as a tie is moved off it by one step where its
+//     own remainder, exact there, is not 0.  A division per element was the
+//     limit: 27.8 us instead of 21.4 for 8192 x 4096 bf16.
 // A NaN stays NaN and leaves its block's scale alone; an infinity takes the
 // largest finite value's scale and saturates.
 #pragma once
@@ -28,10 +30,24 @@ __device__ __forceinline__ int scale_exp_448(float a) {
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
-// n / d with r = 1 / d rounded to nearest; infinities and NaN as n r.
-__device__ __forceinline__ float fp8_quotient(float n, float d, float r) {
-  const float q = n * r;
-  return fabsf(q) < 1e30f ? fmaf(fmaf(-q, d, n), r, q) : q;
+// 0.875 x / d with r = 1 / d rounded to nearest; infinities and NaN as 0.875 x r.
+// WIDE: x has more than 16 bits.
+template <bool WIDE>
+__device__ __forceinline__ float fp8_quotient(float x, float d, float r) {
+  const float n = 0.875f * x;
+  float q = n * r;
+  if (!(fabsf(q) < 1e30f)) return q;
+  const float lo = WIDE ? fmaf(0.875f, x, -n) : 0.f;
+  q = WIDE ? fmaf(fmaf(-q, d, n) + lo, r, q) : fmaf(fmaf(-q, d, n), r, q);
+  if constexpr (WIDE) {
+    // E4M3 values and ties have at most five significant bits
+    const int b = __float_as_int(q);
+    if ((b & 0x7ffff) == 0) {
+      const float rem = fmaf(-q, d, n) + lo;
+      if (rem != 0.f) q = __int_as_float(b + ((__float_as_int(rem) ^ b) < 0 ? -1 : 1));
+    }
+  }
+  return q;
 }
 // The block's a over the 16 lanes that hold it, eight columns each.
 __device__ __forceinline__ float fp8_amax(const float (&v)[8]) {
@@ -49,11 +65,12 @@ __device__ __forceinline__ uint2 fp8_codes_pow2(const float (&v)[8], int e) {
                     e4m3x2(v[4] * inv, v[5] * inv) | (e4m3x2(v[6] * inv, v[7] * inv) << 16));
 }
 // ... and with the scale a / 448: 448 x / a = (0.875 x) / (a / 512), a / 512 exact.
+template <bool WIDE>
 __device__ __forceinline__ uint2 fp8_codes_fp32(const float (&v)[8], float a) {
   const float d = a * 0.001953125f, r = __frcp_rn(d);
   float q[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = fp8_quotient(0.875f * v[j], d, r);
+  for (int j = 0; j < 8; ++j) q[j] = fp8_quotient<WIDE>(v[j], d, r);
   return make_uint2(e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16), e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16));
 }
 __device__ __forceinline__ float fp8_scale_fp32(float a) { return __fdiv_rn(a, 448.f); }
