@@ -243,12 +243,26 @@ __device__ __forceinline__ void load_row(const T* row, int E, float (&v)[NV][4])
   }
 }
 
-// softplus(l) and e = exp(-|l|).  log1p(e) = 2 atanh(z), z = e / (2 + e) <=
-// 1/3, by its power series in z^2 <= 1/9: the first term left out is below
-// 1.5e-8 of the sum, and unlike log(1 + e) it keeps its digits as e goes to 0.
-__device__ __forceinline__ float softplus_e(float l, float* e_out) {
-  const float e = __expf(-fabsf(l));
-  const float z = __fdividef(e, 2.f + e), q = z * z;
+// exp(x) = 2^(x log2 e), the rounding error of the product put back (log2 e in
+// two parts, Cody and Waite 1980): within 6 2^-24 for every x.  The hardware's
+// 2^t of the product alone is off by up to 60 2^-24 at x = -86.
+__device__ __forceinline__ float exp_fast(float x) {
+  const float t = x * 1.4426950216f;
+  float lo = fmaf(x, 1.9259629911e-8f, fmaf(x, 1.4426950216f, -t));
+  if (!(fabsf(t) < 256.f)) lo = 0.f;   // 0, infinity or NaN, whatever the rest
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return fmaf(r, lo * 0.69314718056f, r);
+}
+// sqrt(softplus(l)) = h sqrt(u): for l < 0, h = exp(l / 2) and u = log1p(e) / e
+// with e = h^2; for l >= 0, h = 1 and u = l + log1p(e), e = exp(-l).  So a score
+// keeps its digits down to exp(l / 2) = 2^-126, where softplus(l) itself has
+// long left the range of fp32.  log1p(e) = 2 atanh(z), z = e / (2 + e) <= 1/3,
+// by its power series in z^2 <= 1/9: the first term left out is below 1.5e-8 of
+// the sum, and unlike log(1 + e) it keeps its digits as e goes to 0.
+__device__ __forceinline__ float softplus_root(float l, float* u, float* e_out) {
+  const float h = exp_fast(-0.5f * fabsf(l)), e = h * h;
+  const float w = __fdividef(1.f, 2.f + e), z = e * w, q = z * z;
   float s = 1.f / 13.f;
   s = fmaf(s, q, 1.f / 11.f);
   s = fmaf(s, q, 1.f / 9.f);
@@ -256,38 +270,38 @@ __device__ __forceinline__ float softplus_e(float l, float* e_out) {
   s = fmaf(s, q, 1.f / 5.f);
   s = fmaf(s, q, 1.f / 3.f);
   s = fmaf(s, q, 1.f);
+  const float ratio = 2.f * w * s;
   *e_out = e;
-  return fmaf(2.f * z, s, fmaxf(l, 0.f));
+  *u = l >= 0.f ? fmaf(e, ratio, l) : ratio;
+  return l >= 0.f ? 1.f : h;   // a NaN stays one in h
 }
-// Score of a logit (softmax: relative to the row maximum mx).  The fast
-// exponential, quotient and root are each within a few 2^-23 (the exponential
-// 1.2 |l| 2^-24 more), far below the 2^-8 or so that a 1 % change of a loss
-// weight means; the library's exact ones made the kernel compute-bound.
+// Score of a logit (softmax: relative to the row maximum mx).  The exponential,
+// the fast quotient and the root are each within a few 2^-23; the library's
+// exact ones made the kernel compute-bound.
 template <int SF>
 __device__ __forceinline__ float score_of(float l, float mx) {
   if constexpr (SF == DSV4_SCORE_SOFTMAX) {
-    return __expf(l - mx);
+    return exp_fast(l - mx);
   } else if constexpr (SF == DSV4_SCORE_SIGMOID) {
-    return __fdividef(1.f, 1.f + __expf(-l));
+    return __fdividef(1.f, 1.f + exp_fast(-l));
   } else {
-    float e;
-    const float sp = softplus_e(l, &e);
-    return sp > 0.f ? sp * rsqrtf(sp) : sp;   // sp: 0 or NaN
+    float u, e;
+    const float h = softplus_root(l, &u, &e);
+    return h * (u * rsqrtf(u));
   }
 }
 // dscore / dlogit.
 template <int SF>
 __device__ __forceinline__ float score_slope(float l, float mx) {
   if constexpr (SF == DSV4_SCORE_SOFTMAX) {
-    return __expf(l - mx);
+    return exp_fast(l - mx);
   } else if constexpr (SF == DSV4_SCORE_SIGMOID) {
-    const float e = __expf(-fabsf(l)), d = 1.f + e;   // s (1 - s) = e / (1 + e)^2, either sign of l
+    const float e = exp_fast(-fabsf(l)), d = 1.f + e;   // s (1 - s) = e / (1 + e)^2, either sign of l
     return __fdividef(e, d * d);
   } else {
-    float e;
-    const float sp = softplus_e(l, &e);
-    const float sg = __fdividef(l >= 0.f ? 1.f : e, 1.f + e);
-    return sp > 0.f ? 0.5f * sg * rsqrtf(sp) : sp;
+    float u, e;   // sigma / (2 score), sigma = h^2 / (1 + e)
+    const float h = softplus_root(l, &u, &e);
+    return __fdividef(0.5f * h, 1.f + e) * rsqrtf(u);
   }
 }
 
@@ -301,9 +315,9 @@ template <bool VEC, int NV>
 struct GRow {
   int seq = -1;
   float g[NV][4];
-  __device__ __forceinline__ void from_counts(int s, int2 info, const int* hist, bool global, int E) {
+  __device__ __forceinline__ void from_counts(int s, int2 info, const int* hist, bool global, int E, float scale) {
     seq = s;
-    const float c = g_factor(info, E);
+    const float c = scale * g_factor(info, E);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -327,7 +341,7 @@ struct GRow {
 // all its warps (each warp reading it from L2 made the 1 KB of a batch's only
 // sequence the limit: 59 us instead of 31).  Returns that sequence.  `state`:
 // lanes 0 .. tok - 1 hold the sequences of the warp's rows.
-__device__ __forceinline__ int share_g(const BalanceParams& p, int mine, float* gs, int* first) {
+__device__ __forceinline__ int share_g(const BalanceParams& p, int mine, float* gs, int* first, float scale) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t some = __ballot_sync(0xffffffffu, mine >= 0);
   const int s = __shfl_sync(0xffffffffu, mine, some ? __ffs(some) - 1 : 0);
@@ -337,7 +351,7 @@ __device__ __forceinline__ int share_g(const BalanceParams& p, int mine, float* 
   for (int w = 0; w < BL_WARPS; ++w)
     if (s0 < 0) s0 = first[w];
   if (s0 >= 0) {
-    const float c = g_factor(__ldcg(&p.info[s0]), p.E);
+    const float c = scale * g_factor(__ldcg(&p.info[s0]), p.E);
     for (int e = threadIdx.x; e < p.E; e += BL_THREADS) gs[e] = c * (float)__ldcg(&p.hist[(int64_t)s0 * p.E + e]);
   }
   __syncthreads();
@@ -441,7 +455,7 @@ __global__ void __launch_bounds__(BL_THREADS, NV <= 2 ? BL_CTAS : 1) balance_for
   griddep_wait();
   griddep_launch();
   const int mine = lane < n ? __float_as_int(__ldcg(&p.rows[t0 + lane].w)) : -1;
-  const int s0 = share_g(p, mine, gs, redi);
+  const int s0 = share_g(p, mine, gs, redi, 1.f);
   GRow<VEC, NV> gr;
   float sum = 0.f;
   float4 state = make_float4(0.f, 0.f, 0.f, __int_as_float(mine));   // lane i: row t0 + i
@@ -471,7 +485,7 @@ __global__ void __launch_bounds__(BL_THREADS, NV <= 2 ? BL_CTAS : 1) balance_for
         if (s[r] < 0) continue;
         if (s[r] != gr.seq) {
           if (s[r] == s0) gr.from_shared(s[r], gs, p.E);
-          else gr.from_counts(s[r], __ldcg(&p.info[s[r]]), p.hist + (int64_t)s[r] * p.E, true, p.E);
+          else gr.from_counts(s[r], __ldcg(&p.info[s[r]]), p.hist + (int64_t)s[r] * p.E, true, p.E, 1.f);
         }
         float m1[1], z1[1], d1[1];
         rows_forward<SF, VEC, NV, 1>(v + r, gr, m1, z1, d1);
@@ -540,7 +554,7 @@ __global__ void __launch_bounds__(BL_SMALL_THREADS) balance_forward_small_kernel
     const int s = row_seq[t];
     float mx = 0.f, zi = 0.f, d = 0.f;
     if (s >= 0) {
-      if (s != gr.seq) gr.from_counts(s, info[s], hist + s * p.E, false, p.E);
+      if (s != gr.seq) gr.from_counts(s, info[s], hist + s * p.E, false, p.E, 1.f);
       float m1[1], z1[1], d1[1];
       rows_forward<SF, VEC, NV, 1>(&v, gr, m1, z1, d1);
       mx = m1[0], zi = z1[0], d = d1[0];
@@ -588,7 +602,7 @@ __global__ void __launch_bounds__(BL_THREADS, NV <= 2 ? BL_CTAS : 1) balance_bac
   const float4 state = lane < n ? __ldcg(&p.rows[t0 + lane]) : make_float4(0.f, 0.f, 0.f, __int_as_float(-1));
   const int q = __ldcg(&p.head[0]);
   const float c = q ? p.alpha / (float)q * __ldcg(p.up) : 0.f;
-  const int s0 = share_g(p, __float_as_int(state.w), gs, first);
+  const int s0 = share_g(p, __float_as_int(state.w), gs, first, c);
   GRow<VEC, NV> gr;
 #pragma unroll 1
   for (int b = 0; b < n; b += BATCH) {
@@ -604,18 +618,19 @@ __global__ void __launch_bounds__(BL_THREADS, NV <= 2 ? BL_CTAS : 1) balance_bac
     for (int r = 0; r < BATCH; ++r) {
       if (b + r >= n) break;
       const float mx = __shfl_sync(0xffffffffu, state.x, (b + r) & 31);
-      const float zc = c * __shfl_sync(0xffffffffu, state.y, (b + r) & 31);
-      const float d = __shfl_sync(0xffffffffu, state.z, (b + r) & 31);
+      // c goes with g and d: c / sum would leave fp32 where a row's scores are small
+      const float zi = __shfl_sync(0xffffffffu, state.y, (b + r) & 31);
+      const float d = c * __shfl_sync(0xffffffffu, state.z, (b + r) & 31);
       const int s = __float_as_int(__shfl_sync(0xffffffffu, state.w, (b + r) & 31));
       if (s >= 0) {
         if (s != gr.seq) {
           if (s == s0) gr.from_shared(s, gs, p.E);
-          else gr.from_counts(s, __ldcg(&p.info[s]), p.hist + (int64_t)s * p.E, true, p.E);
+          else gr.from_counts(s, __ldcg(&p.info[s]), p.hist + (int64_t)s * p.E, true, p.E, c);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v[r][i][j] = zc * score_slope<SF>(v[r][i][j], mx) * (gr.g[i][j] - d);
+          for (int j = 0; j < 4; ++j) v[r][i][j] = zi * score_slope<SF>(v[r][i][j], mx) * (gr.g[i][j] - d);
       } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) v[r][i][0] = v[r][i][1] = v[r][i][2] = v[r][i][3] = 0.f;
