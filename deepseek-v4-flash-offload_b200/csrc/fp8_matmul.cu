@@ -45,6 +45,11 @@ constexpr int F_GROUP = 4;             // k-tiles per scale group
 constexpr int F_SLOTS = 4;             // scale groups in flight
 constexpr int F_EPI_WARP0 = 4;
 constexpr int F_MAX_SMEM = 227 * 1024;        // a CTA's opt-in limit
+constexpr int F_SM_SMEM = 228 * 1024;         // an SM's, 1 KB of which each CTA takes beside its own
+constexpr int F_MIN_SMEM = 92 * 1024;         // every kernel here takes more
+// Whether two CTAs of these kernels, one of `smem` bytes and any other, never
+// share an SM; else each may take half of the SM's 512 TMEM columns.
+constexpr bool alone_on_sm(int smem) { return smem + F_MIN_SMEM + 2 * 1024 > F_SM_SMEM; }
 constexpr int64_t F_MAX_M = 65535LL * 128;   // grid y, in tiles of 128 rows
 
 // Set by a kernel whose bounded wait ran out; read by dsv4_fp8_status.
@@ -331,7 +336,8 @@ struct FCfg {
   // these CTAs fit an SM (shared memory), and either both take at most half
   // of the 512 columns or one leaves no room for the other.  (The routed
   // layer's kernels with TMEM take 176 KB or more: none shares an SM with these.)
-  static_assert(SMEM > 76 * 1024 && (TMEM_COLS <= 256 || SMEM > 134 * 1024), "two CTAs share an SM's TMEM");
+  static_assert(SMEM >= F_MIN_SMEM && 3 * (F_MIN_SMEM + 1024) > F_SM_SMEM, "at most two CTAs per SM");
+  static_assert(TMEM_COLS <= 256 || alone_on_sm(SMEM), "two CTAs share an SM's TMEM");
 };
 
 // Eight columns of a row of x from column c (zeros past the end of K).
@@ -765,6 +771,7 @@ struct LCfg {
   // than the block is launched with
   static constexpr int REGS_ISSUE = 56, REGS_EPI = 224, REGS_LAUNCH = 168;
   static_assert(REGS_ISSUE * 128 + REGS_EPI * EPI_WARPS * 32 <= REGS_LAUNCH * THREADS, "register split");
+  static_assert(SMEM >= F_MIN_SMEM && alone_on_sm(SMEM), "takes all 512 TMEM columns");
 };
 
 struct LTile {
