@@ -244,15 +244,15 @@ __device__ __forceinline__ void load_row(const T* row, int E, float (&v)[NV][4])
 }
 
 // exp(x) = 2^(x log2 e), the rounding error of the product put back (log2 e in
-// two parts, Cody and Waite 1980): within 6 2^-24 for every x.  The hardware's
-// 2^t of the product alone is off by up to 60 2^-24 at x = -86.
+// two parts, Cody and Waite 1980): within 6 2^-24 for results between 2^-126
+// and 2^126.  The hardware's 2^t of the product alone is off by up to 60 2^-24
+// at x = -86.  Beyond, 2^t as it is: 0, infinity or NaN have no error to put back.
 __device__ __forceinline__ float exp_fast(float x) {
   const float t = x * 1.4426950216f;
-  float lo = fmaf(x, 1.9259629911e-8f, fmaf(x, 1.4426950216f, -t));
-  if (!(fabsf(t) < 256.f)) lo = 0.f;   // 0, infinity or NaN, whatever the rest
+  const float lo = fmaf(x, 1.9259629911e-8f, fmaf(x, 1.4426950216f, -t));
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
-  return fmaf(r, lo * 0.69314718056f, r);
+  return fabsf(t) < 126.f ? fmaf(r, lo * 0.69314718056f, r) : r;
 }
 // sqrt(softplus(l)) = h sqrt(u): for l < 0, h = exp(l / 2) and u = log1p(e) / e
 // with e = h^2; for l >= 0, h = 1 and u = l + log1p(e), e = exp(-l).  So a score
