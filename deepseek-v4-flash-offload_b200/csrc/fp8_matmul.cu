@@ -165,8 +165,10 @@ __device__ __forceinline__ uint32_t map_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
 }
-// Arrival that publishes nothing (an accumulator has been read: its values are
-// in registers).  A release at cluster scope here, and an acquire in the wait
+// Arrival that publishes nothing in memory (an accumulator has been read: its
+// values are in registers).  What it orders, the loads from TMEM before the
+// leader's next MMA into it, the tcgen05 fences on both sides of each wait and
+// arrival order; a release at cluster scope here, and an acquire in the wait
 // for it, cost 1.1 us per k-tile together.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
@@ -995,6 +997,10 @@ __global__ void __launch_bounds__(LCfg<E8>::THREADS, 1)
       for (int u = 0; u < uses; ++u) {
         const int ab = u % C::NACC;
         if (!warp_wait(&accempty[ab], (uint32_t)(u / C::NACC) & 1u, err)) break;
+        // the epilogue's tcgen05.ld -> fence, arrival | wait, fence -> fence,
+        // arrival | wait, fence -> the leader's MMA: every link has its fences
+        tc_fence_after();
+        tc_fence_before();
         if (lane == 0) mbar_arrive_cluster_relaxed(map_rank(&accempty[ab], 0));
         __syncwarp();
       }
