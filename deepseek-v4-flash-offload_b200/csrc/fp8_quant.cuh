@@ -34,20 +34,17 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
 // WIDE: x has more than 16 bits.
 template <bool WIDE>
 __device__ __forceinline__ float fp8_quotient(float x, float d, float r) {
-  const float n = 0.875f * x;
-  float q = n * r;
-  if (!(fabsf(q) < 1e30f)) return q;
-  const float lo = WIDE ? fmaf(0.875f, x, -n) : 0.f;
-  q = WIDE ? fmaf(fmaf(-q, d, n) + lo, r, q) : fmaf(fmaf(-q, d, n), r, q);
-  if constexpr (WIDE) {
-    // E4M3 values and ties have at most five significant bits
-    const int b = __float_as_int(q);
-    if ((b & 0x7ffff) == 0) {
-      const float rem = fmaf(-q, d, n) + lo;
-      if (rem != 0.f) q = __int_as_float(b + ((__float_as_int(rem) ^ b) < 0 ? -1 : 1));
-    }
-  }
-  return q;
+  const float n = 0.875f * x, q = n * r;
+  const float rem = WIDE ? fmaf(-q, d, n) + fmaf(0.875f, x, -n) : fmaf(-q, d, n);
+  return fabsf(q) < 1e30f ? fmaf(rem, r, q) : q;
+}
+// E4M3 values and ties have at most five significant bits.
+__device__ __forceinline__ bool fp8_maybe_tie(float q) { return (__float_as_int(q) & 0x7ffff) == 0; }
+// q moved by one step towards the real 0.875 x / d, if that is another number.
+__device__ __forceinline__ float fp8_off_tie(float q, float x, float d) {
+  const float n = 0.875f * x, rem = fmaf(-q, d, n) + fmaf(0.875f, x, -n);
+  if (rem == 0.f || !(fabsf(q) < 1e30f)) return q;
+  return __int_as_float(__float_as_int(q) + ((__float_as_int(rem) ^ __float_as_int(q)) < 0 ? -1 : 1));
 }
 // The block's a over the 16 lanes that hold it, eight columns each.
 __device__ __forceinline__ float fp8_amax(const float (&v)[8]) {
@@ -69,8 +66,17 @@ template <bool WIDE>
 __device__ __forceinline__ uint2 fp8_codes_fp32(const float (&v)[8], float a) {
   const float d = a * 0.001953125f, r = __frcp_rn(d);
   float q[8];
+  bool tie = false;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = fp8_quotient<WIDE>(v[j], d, r);
+  for (int j = 0; j < 8; ++j) {
+    q[j] = fp8_quotient<WIDE>(v[j], d, r);
+    if constexpr (WIDE) tie |= fp8_maybe_tie(q[j]);
+  }
+  if (WIDE && tie) {   // one element in 2^19, and zeros
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (fp8_maybe_tie(q[j])) q[j] = fp8_off_tie(q[j], v[j], d);
+  }
   return make_uint2(e4m3x2(q[0], q[1]) | (e4m3x2(q[2], q[3]) << 16), e4m3x2(q[4], q[5]) | (e4m3x2(q[6], q[7]) << 16));
 }
 __device__ __forceinline__ float fp8_scale_fp32(float a) { return __fdiv_rn(a, 448.f); }
