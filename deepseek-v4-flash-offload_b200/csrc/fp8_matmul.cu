@@ -15,7 +15,8 @@
 // fp32 scales: kind::f8f6f4 into a ring of TMEM accumulators, one k-tile each;
 //   the epilogue warps add as * bs times each partial sum to fp32 registers.
 //   Handing an accumulator over (commit, load, release) takes about as long as
-//   three k-tiles' MMAs, hence four of them.
+//   three k-tiles' MMAs: four of them with few rows, two wider ones in the
+//   pair kernel.
 //
 // Measured (device, graph replay): 1 x 2048 x 4096 5.0 us, 64 x 4096 x 4096 7.4
 // us, 2048 x 4096 x 4096 29 us, 8192 x 8192 x 4096 206 us (2.67 PFLOP/s) with
@@ -1225,9 +1226,9 @@ int launch_cluster(K k, dim3 grid, int threads, int smem, dim3 cluster, cudaStre
 // The occupancy query answers for one CTA per SM: it is asked with the largest
 // shared memory.
 template <typename K>
-int fitting_cluster(K k, int threads, int resident, int64_t tiles, int want, int dev, std::atomic<int> (&known)[9]) {
+int fitting_cluster(K k, int threads, int resident, int64_t tiles, int want, int dev, std::atomic<int> (&known)[64][9]) {
   for (; want > 1; --want) {
-    int n = dev == 0 ? known[want].load(std::memory_order_relaxed) : 0;
+    int n = dev < 64 ? known[dev][want].load(std::memory_order_relaxed) : 0;
     if (n == 0) {
       cudaLaunchConfig_t cfg = {};
       cfg.gridDim = dim3(1, 1, (unsigned)want);
@@ -1245,21 +1246,34 @@ int fitting_cluster(K k, int threads, int resident, int64_t tiles, int want, int
         n = 0;
       }
       if (n == 0) n = -1;
-      if (dev == 0) known[want].store(n, std::memory_order_relaxed);
+      if (dev < 64) known[dev][want].store(n, std::memory_order_relaxed);
     }
     if ((int64_t)n * resident >= tiles) break;
   }
   return want;
 }
+// The few-row kernel made ready on `dev`, and *cluster reduced to the size that fits.
+template <int BN, bool E8, bool A_MN, bool FUSE>
+int fit_small(int64_t tiles, int dev, int* cluster) {
+  using C = FCfg<BN, E8, FUSE>;
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> fits[64][9];
+  auto k = fp8_matmul_kernel<BN, E8, A_MN, FUSE>;
+  if (int rc = prepare_kernel(k, F_MAX_SMEM, 0, dev, done)) return rc;
+  *cluster = fitting_cluster(k, C::THREADS, C::RESIDENT, tiles, *cluster, dev, fits);
+  return DSV4_OK;
+}
+template <int BN>
+int fit_fused(bool e8, bool a_mn, int64_t tiles, int dev, int* cluster) {
+  if (e8) return a_mn ? fit_small<BN, true, true, true>(tiles, dev, cluster) : fit_small<BN, true, false, true>(tiles, dev, cluster);
+  return a_mn ? fit_small<BN, false, true, true>(tiles, dev, cluster) : fit_small<BN, false, false, true>(tiles, dev, cluster);
+}
 template <int BN, bool E8, bool A_MN, bool FUSE>
 int launch_small(const CUtensorMap& tw, const CUtensorMap& tx, const Fp8Params& p, int want, int dev, cudaStream_t st) {
   using C = FCfg<BN, E8, FUSE>;
-  static std::atomic<uint64_t> done{0};
-  static std::atomic<int> fits[9];
   auto k = fp8_matmul_kernel<BN, E8, A_MN, FUSE>;
-  if (int rc = prepare_kernel(k, F_MAX_SMEM, 0, dev, done)) return rc;
   const int64_t nt = (p.N + F_BM - 1) / F_BM, mt = (p.M + BN - 1) / BN;
-  want = fitting_cluster(k, C::THREADS, C::RESIDENT, nt * mt, want, dev, fits);
+  if (int rc = fit_small<BN, E8, A_MN, FUSE>(nt * mt, dev, &want)) return rc;
   const int per = k_share(p.kb, want);
   const unsigned split = (unsigned)((p.kb + per - 1) / per);
   return launch_cluster(k, dim3((unsigned)nt, (unsigned)mt, split), C::THREADS, C::SMEM, dim3(1, 1, split), st, tw, tx,
@@ -1351,12 +1365,23 @@ static int fp8_matmul_run(const uint8_t* a, int64_t lda, const void* as, const u
 // 4096 x 4096: 6.4 | 8.2, 64 x 4096 x 2048 (4 k-tiles): 7.7 | 8.1, 64 x 8192 x
 // 8192 (32 k-tiles): 28 | 17; fp32: 1 x 2048 x 4096: 6.3 | 6.6, 64 x 4096 x
 // 2048: 10.4 | 8.5.
-static bool linear_fuses(const void* x, int x_dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, bool e8, int sms) {
-  if (m > 64 || x_dtype != DSV4_DT_BF16 || k % 8 || (uintptr_t)x % 16 || ldx % 8) return false;
-  const int split = fp8_shape(m, n, sms).split, per = k_share((int)((k + F_BK - 1) / F_BK), split);
-  if (m <= 16) return per <= (e8 ? 8 : 4);
+// Only where the fused kernel's clusters fit at the full size: the other one,
+// of which as many CTAs or more share an SM, then splits K the same way, and
+// the sums have the same order.
+static bool linear_fuses(const void* x, int x_dtype, int64_t ldx, int64_t m, int64_t n, int64_t k, bool e8, bool a_mn,
+                         int dev) {
+  const int sms = sm_count(dev);
+  if (sms <= 0 || m > 64 || x_dtype != DSV4_DT_BF16 || k % 8 || (uintptr_t)x % 16 || ldx % 8) return false;
+  const Fp8Shape c = fp8_shape(m, n, sms);
+  const int per = k_share((int)((k + F_BK - 1) / F_BK), c.split);
   // above 32 rows one CTA fits an SM, and few clusters of more than four do
-  return e8 && per <= 4 && (m <= 32 || split <= 4);
+  if (m <= 16 ? per > (e8 ? 8 : 4) : !(e8 && per <= 4 && (m <= 32 || c.split <= 4))) return false;
+  const int64_t tiles = (n + F_BM - 1) / F_BM;
+  int fits = c.split;
+  const int rc = c.bn == 16   ? fit_fused<16>(e8, a_mn, tiles, dev, &fits)
+                 : c.bn == 32 ? fit_fused<32>(e8, a_mn, tiles, dev, &fits)
+                              : fit_fused<64>(e8, a_mn, tiles, dev, &fits);
+  return rc == DSV4_OK && fits == c.split;
 }
 static int fp8_linear_fused(const void* x, int64_t ldx, const uint8_t* w, int64_t ldw, const void* ws,
                             int scale_type, bool trans_w, int64_t m, int64_t n, int64_t k, void* y, int64_t ldy,
@@ -1447,7 +1472,7 @@ extern "C" int dsv4_fp8_linear(const void* x, int32_t x_dtype, int64_t ldx, cons
   DeviceScope dev;
   if (int rc = dev.enter(x)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  if (linear_fuses(x, x_dtype, ldx, m, n, k, scale_type == DSV4_SCALE_E8M0, sm_count(dev.device)))
+  if (linear_fuses(x, x_dtype, ldx, m, n, k, scale_type == DSV4_SCALE_E8M0, trans_w == 0, dev.device))
     return fp8_linear_fused(x, ldx, w, ldw, w_scale, scale_type, trans_w != 0, m, n, k, y, ldy, dev.device, st);
   uint8_t* q = static_cast<uint8_t*>(workspace);
   uint8_t* s = q + linear_scale_offset(m, k);

@@ -105,3 +105,53 @@ def test_balance_rows_of_small_scores(ops, fn, l, t):
     s = balance64(lg.double(), fn)
     p = s / s.sum(1, keepdim=True)
     assert ((grad.double() - gw).abs() <= tol * 65536.0 * p * 16 / t).all()
+
+
+@pytest.mark.parametrize("n", [2304, 2432, 4480, 4608, 4736])
+@pytest.mark.parametrize("m", [16, 32, 64])
+@pytest.mark.parametrize("k", [512, 2048, 4096])
+def test_fp8_linear_is_its_parts_where_clusters_fill_the_gpu(ops, m, n, k):
+    """As many clusters as the SMs take, and one more: a cluster size that
+    does not fit is made smaller, in one launch as in two."""
+    g = gen(m + n + k)
+    w = (torch.randn((n, k), generator=g, device="cuda") * 100).clamp(-448, 448).to(F8)
+    ws = torch.exp2(torch.randint(-15, -8, (-(-n // 128), -(-k // 128)), generator=g, device="cuda").float()).to(E8)
+    x = torch.randn((m, k), generator=g, device="cuda").bfloat16()
+    want = ops.fp8_matmul(*ops.act_quant(x, 128, "ue8m0", E8), w, ws)
+    assert torch.equal(ops.fp8_linear(x, w, ws), want)
+    ops.fp8_status()
+
+
+def test_fp8_operators_beside_the_routed_layer(ops):
+    """Clusters that split K, CTA pairs, the routed layer and the prompt's
+    router on four streams together: the bits of a serial run."""
+    from dsv4_plugin import synthetic as S
+    from helpers import SyntheticLayer, bf16_tensor
+    cfg = S.CFG0
+    layer = SyntheticLayer(cfg)
+    xt = bf16_tensor(S.make_tokens(cfg, 3, 512))
+    gate = torch.from_numpy(layer.gate_w).cuda()
+    plan = ops.MoEPlan(cfg.hidden, cfg.inter, cfg.n_experts, cfg.topk, 512, cfg.swiglu_limit, layer.arena)
+    w, idx = ops.route_topk(xt, gate, None, cfg.topk, cfg.score_func, cfg.renormalize)
+    g = gen(1)
+    f8 = lambda n, k: ((torch.randn((n, k), generator=g, device="cuda") * 100).clamp(-448, 448).to(F8),  # noqa: E731
+                       torch.full((-(-n // 128), -(-k // 128)), 2.0 ** -10, device="cuda"))
+    big, small = f8(2304, 2048), f8(1024, 4096)
+    xb = torch.randn((1500, 2048), generator=g, device="cuda").bfloat16()
+    xs = torch.randn((100, 4096), generator=g, device="cuda").bfloat16()
+    calls = [lambda: ops.fp8_linear(xb, *big), lambda: ops.fp8_linear(xs, *small),
+             lambda: plan.forward(xt, w, idx, layer.slot_of).clone(),
+             lambda: ops.route_topk(xt, gate, None, cfg.topk, cfg.score_func, cfg.renormalize)[0]]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[] for _ in calls]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    ops.fp8_status()
+    plan.status()
+    for i, w0 in enumerate(want):
+        assert all(torch.equal(y, w0) for y in got[i])
