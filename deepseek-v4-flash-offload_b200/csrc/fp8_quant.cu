@@ -8,7 +8,8 @@
 // 8; a warp has eight blocks in flight before the first reduction.  Rows that
 // do not start on 16 bytes take one element per load, neighbours across the
 // lanes.  Measured: 8192 x 4096 bf16 with E8M0 scales 17.2 us (5.9 TB/s, 91 %
-// of the copy rate), 4095 x 2008 fp32 with fp32 scales 8.3 us.
+// of the copy rate), 4095 x 2008 fp32 with fp32 scales 11.8 us
+// (64 registers for the exact ties, two waves of CTAs).
 #include "capi_internal.h"
 #include "common.cuh"
 #include "fp8_quant.cuh"

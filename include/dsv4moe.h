@@ -120,8 +120,8 @@ int dsv4_act_quant_mxfp4(const void* x_bf16, int64_t rows, int64_t cols, uint8_t
  *   trans_b != 0: b [n, k], b_scale [ceil(n / 128), ceil(k / 128)];
  *   trans_b == 0: b [k, n], b_scale [ceil(k / 128), ceil(n / 128)],
  * row stride ldb bytes; both scales E8M0 bytes or both fp32.  fp32 sums.  a
- * and b start on 16 bytes with row strides that are multiples of 16; k, m
- * and n are any size.
+ * and b start on 16 bytes with row strides that are multiples of 16; k and n
+ * are any size, m is at most 65535 * 128.
  * A device-side wait that runs out is reported by dsv4_fp8_status.
  * ------------------------------------------------------------------------ */
 #define DSV4_DT_BF16 0
@@ -162,7 +162,7 @@ int dsv4_fp8_status(int32_t device, void* stream);
  *   loss = alpha * mean over sequences with tokens of
  *          sum_e f[s, e] * (1 / n[s]) * sum_t p[t, e];
  * counts [n_seqs, n_experts] = c.  A row whose scores are all 0 has p = 0 (a
- * sigmoid below 2^-126, the smallest normal fp32 number, counts as 0); a
+ * score below 2^-126, the smallest normal fp32 number, counts as 0); a
  * NaN or an infinite score makes the loss and its row's gradient NaN.  Picks
  * outside [-1, n_experts) are skipped, and like offsets that descend or
  * leave [0, n_tokens] they set DSV4_EINVAL in *status (device word, may be
